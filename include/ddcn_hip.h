@@ -349,6 +349,80 @@ int ddcn_deform_psroi_pool_backward_f64(const double *grad_out, const double *da
                                         const double *offset, const double *out_count, double *grad_data,
                                         double *grad_offset, const ddcn_roi_geom *g, void *stream);
 
+/* ---------------------------------------------------------------- AdamW over many tensors
+ * Not in the reference (its optimizer is torch.optim.SGD): the update of every parameter tensor of a model in a few
+ * launches, with the two moments in fp32 or in 8-bit codes, and the global gradient norm it may be clipped by.
+ * Element types of parameters and gradients: */
+enum { DDCN_F32 = 0, DDCN_BF16 = 1, DDCN_F16 = 2 };
+
+typedef struct ddcn_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay;
+    double max_norm;   /* clip by the norm behind `grad_norm`; not read when grad_norm is NULL */
+    int step;          /* t >= 1 of the bias corrections 1 - beta^t, for every tensor when `steps` is NULL */
+    int dtype;         /* DDCN_F32 / DDCN_BF16 / DDCN_F16, of parameters and gradients */
+    int bits;          /* of the moments: 32 or 8 */
+    unsigned seed;     /* of the random rounding of 8-bit codes */
+} ddcn_adamw_hyper;
+
+/* Elements of the moments' arena for `count` tensors: tensor i starts at the next multiple of 256 elements behind
+ * tensor i-1.  Negative: DDCN_ERR_*. */
+long long ddcn_adamw_arena(int count, const long long *numels);
+
+/* One step, in place.  `params`, `grads`, `numels` (and `steps`, or NULL) are HOST arrays of `count` entries: device
+ * addresses, element counts, step numbers.  A NULL gradient leaves its tensor and its part of the arena as they were;
+ * a tensor may not be listed twice.  `exp_avg`, `exp_avg_sq`: the arena (fp32, or int8 / uint8 with one fp32 scale per
+ * 256 elements in `exp_avg_scale` / `exp_avg_sq_scale`).  `grad_norm`: one fp32 on the device, or NULL for no clipping;
+ * a norm that is not finite leaves everything as it was.  The arithmetic (fl = one rounding to fp32):
+ *   g' = fl(c g), c = fl(min(1, max_norm / (norm + 1e-6)));  m = fl(b1 m + (1-b1) g');  v = fl(b2 v + ((1-b2) g') g');
+ *   r = fl(sqrt(v));  p <- p (1 - lr wd) - lr / (1 - b1^t) m / (r / sqrt(1 - b2^t) + eps), in fp32, rounded once to the
+ *   parameter's type.
+ * A signed code q stands for m = s q|q|, s = max|m| / 127^2 of its 256 elements; an unsigned one for r = s q^2,
+ * s = max r / 255^2.  |q| = floor(sqrt(x / s) + u) with u in [0, 1) hashed from (seed, place in the arena): unbiased, so
+ * that a moment moves by less than a code per step on average (to nearest, it would stand still); r > 0 keeps q >= 1, so
+ * that no update divides by a second moment that rounding has made zero.  Blocks whose largest |m| is below 2^-100 are
+ * zero; one that holds a NaN or an infinity becomes NaN. */
+int ddcn_adamw_step(int count, const unsigned long long *params, const unsigned long long *grads,
+                    const long long *numels, const int *steps, void *exp_avg, void *exp_avg_sq, float *exp_avg_scale,
+                    float *exp_avg_sq_scale, const float *grad_norm, const ddcn_adamw_hyper *hyper, void *stream);
+
+/* The fp32 values that 8-bit moments stand for; `numel` a multiple of 256 (an arena). */
+int ddcn_adamw_moments(const void *exp_avg, const void *exp_avg_sq, const float *exp_avg_scale,
+                       const float *exp_avg_sq_scale, float *m, float *v, long long numel, void *stream);
+
+/* out[0] = sqrt(sum of squares) over every element of `count` tensors (`dtypes`: one of the element types each), summed
+ * in fp64 in a fixed order and rounded once.  `workspace`: ddcn_grad_norm_workspace_bytes(), 16-byte aligned. */
+size_t ddcn_grad_norm_workspace_bytes(int count, const long long *numels);
+int ddcn_grad_norm(int count, const unsigned long long *grads, const long long *numels, const int *dtypes, float *out,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------- products in 8-bit integers
+ * Not in the reference: linear layers and 1x1 convolutions at inference, y = s_token s_channel sum_k q w (+ bias, ReLU).
+ * A token is a row of `x` (a RoI, a channels-last pixel) or a pixel of an NCHW map; its k values are rounded to int8 on
+ * the way: s = max(max|x|, 2^-96) / 127, q = round to nearest even of x * (127 / max(max|x|, 2^-96)), fp32.  A token that
+ * holds a NaN or an infinity gives NaN in all of its outputs.  The sum is exact (int32).
+ * Token t = (image i, row h, column w) of a grid images x rows x cols reads x[i*si + h*sh + w*sw + k*sk] and writes
+ * y[i*channels*rows*cols + n*rows*cols + h*cols + w] (nchw) or y[t*channels + n] (not nchw); a matrix of M rows is the grid
+ * (1, M, 1) with sh = its row stride, sk = 1. */
+typedef struct ddcn_int8_geom {
+    int images, rows, cols;        /* token grid; tokens = images*rows*cols (0 is allowed: nothing is launched) */
+    int k;                         /* values of a token (1 .. 131072) */
+    int channels;                  /* output channels */
+    int nchw;                      /* output layout */
+    int dtype;                     /* DDCN_F32 / DDCN_BF16 / DDCN_F16 of x */
+    int out_dtype;                 /* of y */
+    int relu;
+    long long si, sh, sw, sk;      /* strides of x in elements */
+    long long ldw;                 /* row stride of the weights in bytes */
+} ddcn_int8_geom;
+
+size_t ddcn_int8_workspace_bytes(const ddcn_int8_geom *g);
+/* weight: int8 [channels][ldw] (k of each row are read), weight_scale fp32 [channels], bias fp32 [channels] or NULL.
+ * `workspace`: ddcn_int8_workspace_bytes(), 256-byte aligned. */
+int ddcn_int8_product(const void *x, const void *weight, const float *weight_scale, const float *bias, void *y,
+                      void *workspace, size_t workspace_bytes, const ddcn_int8_geom *g, void *stream);
+/* The rounding alone: q int8 [tokens][ldq] (ldq >= k; bytes from k to ldq are zeroed), scale fp32 [tokens]. */
+int ddcn_int8_quantize(const void *x, void *q, long long ldq, float *scale, const ddcn_int8_geom *g, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

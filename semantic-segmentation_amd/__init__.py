@@ -7,12 +7,13 @@ The directory name is hyphenated, so import it with
 from .dcn import (DeformConv, DeformConvPack, ModulatedDeformConv, ModulatedDeformConvPack, DepthawareConv,
                   DepthDeformConvPack, DeformConvFunction, ModulatedDeformConvFunction, DepthawareConvFunction,
                   deform_conv, modulated_deform_conv, depthaware_conv, DeformRoIPooling, DeformRoIPoolingPack,
-                  ModulatedDeformRoIPoolingPack, DeformRoIPoolingFunction, deform_roi_pooling)
+                  ModulatedDeformRoIPoolingPack, DeformRoIPoolingFunction, deform_roi_pooling, quantize_int8, int8_linear,
+                  int8_conv1x1, Int8Linear, Int8Conv1x1)
 
 __all__ = [
     'DeformConv', 'DeformConvPack', 'ModulatedDeformConv', 'ModulatedDeformConvPack', 'DepthawareConv',
     'DepthDeformConvPack', 'DeformConvFunction', 'ModulatedDeformConvFunction', 'DepthawareConvFunction',
     'deform_conv', 'modulated_deform_conv', 'depthaware_conv',
     'DeformRoIPooling', 'DeformRoIPoolingPack', 'ModulatedDeformRoIPoolingPack', 'DeformRoIPoolingFunction',
-    'deform_roi_pooling'
+    'deform_roi_pooling', 'quantize_int8', 'int8_linear', 'int8_conv1x1', 'Int8Linear', 'Int8Conv1x1'
 ]

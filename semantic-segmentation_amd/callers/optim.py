@@ -1,0 +1,309 @@
+"""AdamW over all parameters of a model in a few launches, with the moments in float32 or in 8-bit codes, and the
+global gradient norm it may clip by.  Not in the reference, whose optimizer is torch.optim.SGD (detseg/apis/train.py:64-105);
+the kernels are csrc/ddcn_optim.hip, the arithmetic is written down in include/ddcn_hip.h.
+
+The moments of a step live in one arena per moment: tensor i starts at the next multiple of 256 elements behind tensor
+i - 1 (`adamw_arena` gives the length).  In 8 bits `exp_avg` is int8, `exp_avg_sq` uint8, each with one float32 scale per
+256 elements: 2.03 bytes a parameter instead of 8.  CPU tensors raise NotImplementedError; there is no fallback.
+"""
+import copy
+import ctypes
+from array import array
+from operator import attrgetter
+
+import torch
+
+from ..dcn import _lib
+
+BLOCK = 256
+_Tensor = torch.Tensor
+_dtype_of = attrgetter("dtype")
+
+
+def _address(a):
+    return ctypes.c_void_p(a.buffer_info()[0]) if len(a) else None
+
+
+def _one_device(tensors, name):
+    """Index of the GPU that every tensor lives on."""
+    where = set(map(_Tensor.get_device, tensors))
+    if -1 in where:
+        raise NotImplementedError
+    if len(where) > 1:
+        raise RuntimeError("ddcn: %s are on more than one device" % name)
+    return where.pop()
+
+
+def _check_layout(tensors, name):
+    for t in tensors:
+        if t.layout is not torch.strided:
+            raise RuntimeError("ddcn: %s must be dense tensors, got %s" % (name, t.layout))
+    if not all(map(_Tensor.is_contiguous, tensors)):
+        raise RuntimeError("ddcn: %s tensors have to be contiguous" % name)
+
+
+def adamw_arena(params):
+    """Elements of the arena that holds one moment of `params`."""
+    numels = array("q", map(_Tensor.numel, params))
+    n = _lib.lib().ddcn_adamw_arena(len(numels), _address(numels))
+    if n < 0:
+        _lib.check(n)
+    return n
+
+
+def grad_norm(grads):
+    """sqrt of the sum of squares over all `grads` (entries may be None), a float32 scalar on their GPU: summed in
+    float64 in a fixed order, so that it is the same at every call.  Types may be mixed."""
+    grads = [g.detach() for g in grads if g is not None]
+    if not grads:
+        raise RuntimeError("ddcn: grad_norm needs at least one gradient")
+    dev = _one_device(grads, "gradients")
+    _check_layout(grads, "gradient")
+    try:
+        dtypes = array("i", [_lib.ELEMENT_TYPES[g.dtype] for g in grads])
+    except KeyError as e:
+        raise RuntimeError("ddcn: %s gradients are not supported (float32, float16, bfloat16)" % e) from None
+    pointers, numels = array("Q", map(_Tensor.data_ptr, grads)), array("q", map(_Tensor.numel, grads))
+    L = _lib.lib()
+    nbytes = L.ddcn_grad_norm_workspace_bytes(len(grads), _address(numels))
+    with torch.cuda.device(dev):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device)
+        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        _lib.check(L.ddcn_grad_norm(len(grads), _address(pointers), _address(numels), _address(dtypes), _lib.ptr(out),
+                                    _lib.ptr(ws), nbytes, _lib.current_stream(grads[0].device)))
+    return out
+
+
+def _check_state(name, t, dtype, numel, device):
+    if t.get_device() != device:
+        if not t.is_cuda:
+            raise NotImplementedError
+        raise RuntimeError("ddcn: %s is on another device than the parameters" % name)
+    if t.dtype != dtype or t.numel() != numel or not t.is_contiguous():
+        raise RuntimeError("ddcn: %s has to be a contiguous %s tensor of %d elements, got %s of %d"
+                           % (name, dtype, numel, t.dtype, t.numel()))
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               exp_avg_scale=None, exp_avg_sq_scale=None, seed=0, grad_norm=None, max_norm=None):
+    """One AdamW step over `params` (list of tensors of one type: float32, bfloat16 or float16), in place.
+
+    `grads`: as many tensors of the same shapes and type; None leaves a parameter and its moments as they are.
+    `exp_avg`, `exp_avg_sq`: the arenas (`adamw_arena(params)` elements): float32, or int8 and uint8 with
+    `exp_avg_scale`, `exp_avg_sq_scale` (float32, one per 256 elements) and `seed`, a whole number that should differ
+    from step to step: it drives the unbiased rounding of the codes, and the same seed gives the same codes.
+    `step`: t of the bias corrections, from 1 on, or one for each tensor.  With `max_norm` the gradients are scaled by
+    min(1, max_norm / (grad_norm + 1e-6)), `grad_norm` being a float32 scalar on the GPU (see `grad_norm()`): nothing
+    waits for it, and if it is not finite the step changes nothing.
+
+    Everything else is as in torch.optim.AdamW: p <- p (1 - lr wd) - lr m^ / (sqrt(v^) + eps).  The step number, lr and
+    seed are fixed when the call is made, so it refuses to be captured into a HIP graph."""
+    params, grads = list(params), list(grads)
+    if len(params) != len(grads):
+        raise RuntimeError("ddcn: %d parameters but %d gradients" % (len(params), len(grads)))
+    if not params:
+        return
+    dtype = params[0].dtype
+    if any(g is None for g in grads):
+        given = [g for g in grads if g is not None]
+        mine = [p for p, g in zip(params, grads) if g is not None]
+    else:
+        given, mine = grads, params
+    dev = _one_device(params + given + ([grad_norm] if grad_norm is not None else []), "parameters and gradients")
+    if dtype not in _lib.ELEMENT_TYPES:
+        raise RuntimeError("ddcn: %s parameters are not supported (float32, float16, bfloat16)" % dtype)
+    if set(map(_dtype_of, params)) | set(map(_dtype_of, given)) != {dtype}:
+        raise RuntimeError("ddcn: the parameters and gradients of one step must share a dtype (%s)" % dtype)
+    _check_layout(params, "parameter")
+    _check_layout(given, "gradient")
+    numels = array("q", map(_Tensor.numel, params))
+    if list(map(_Tensor.numel, given)) != (numels.tolist() if given is grads else list(map(_Tensor.numel, mine))):
+        raise RuntimeError("ddcn: a gradient has another number of elements than its parameter")
+    pointers = array("Q", map(_Tensor.data_ptr, params))
+    starts = [a for a, n in zip(pointers, numels) if n]
+    if len(set(starts)) != len(starts):
+        raise RuntimeError("ddcn: a parameter is listed twice")
+    L = _lib.lib()
+    arena = adamw_arena(params)
+    bits = 8 if exp_avg.dtype == torch.int8 else 32
+    _check_state("exp_avg", exp_avg, torch.int8 if bits == 8 else torch.float32, arena, dev)
+    _check_state("exp_avg_sq", exp_avg_sq, torch.uint8 if bits == 8 else torch.float32, arena, dev)
+    if bits == 8:
+        if exp_avg_scale is None or exp_avg_sq_scale is None:
+            raise RuntimeError("ddcn: 8-bit moments need exp_avg_scale and exp_avg_sq_scale")
+        _check_state("exp_avg_scale", exp_avg_scale, torch.float32, arena // BLOCK, dev)
+        _check_state("exp_avg_sq_scale", exp_avg_sq_scale, torch.float32, arena // BLOCK, dev)
+    elif exp_avg_scale is not None or exp_avg_sq_scale is not None:
+        raise RuntimeError("ddcn: float32 moments take no scales")
+    if (max_norm is None) != (grad_norm is None):
+        raise RuntimeError("ddcn: max_norm and grad_norm go together")
+    if grad_norm is not None and (grad_norm.dtype != torch.float32 or grad_norm.numel() != 1):
+        raise RuntimeError("ddcn: grad_norm has to be one float32 value")
+    steps = None
+    if not hasattr(step, "__index__"):
+        steps, step = array("i", step), 1
+        if len(steps) != len(params):
+            raise RuntimeError("ddcn: %d parameters but %d step numbers" % (len(params), len(steps)))
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("ddcn: adamw_step cannot be captured into a HIP graph: a replay would repeat the step number, "
+                           "the learning rate and the seed of the capture")
+    hyper = _lib.AdamwHyper(lr, betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, step,
+                            _lib.ELEMENT_TYPES[dtype], bits, int(seed) & 0xFFFFFFFF)
+    gradients = array("Q", [0 if g is None else g.data_ptr() for g in grads])
+    with torch.cuda.device(dev):
+        _lib.check(L.ddcn_adamw_step(len(params), _address(pointers), _address(gradients), _address(numels),
+                                     None if steps is None else _address(steps), _lib.ptr(exp_avg),
+                                     _lib.ptr(exp_avg_sq), _lib.ptr(exp_avg_scale), _lib.ptr(exp_avg_sq_scale),
+                                     _lib.ptr(grad_norm), hyper, _lib.current_stream(params[0].device)))
+    # the kernels write behind autograd's back: a backward pass that saved one of these must notice
+    torch.autograd.graph.increment_version(mine + [exp_avg, exp_avg_sq] +
+                                           ([exp_avg_scale, exp_avg_sq_scale] if bits == 8 else []))
+
+
+def adamw_moments(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
+    """(m, v) in float32: what the 8-bit codes of two arenas stand for."""
+    dev, n = exp_avg.get_device(), exp_avg.numel()
+    if dev < 0:
+        raise NotImplementedError
+    if n % BLOCK:
+        raise RuntimeError("ddcn: an arena has a multiple of %d elements, got %d" % (BLOCK, n))
+    _check_state("exp_avg", exp_avg, torch.int8, n, dev)
+    _check_state("exp_avg_sq", exp_avg_sq, torch.uint8, n, dev)
+    _check_state("exp_avg_scale", exp_avg_scale, torch.float32, n // BLOCK, dev)
+    _check_state("exp_avg_sq_scale", exp_avg_sq_scale, torch.float32, n // BLOCK, dev)
+    with torch.cuda.device(dev):
+        m = torch.empty(n, dtype=torch.float32, device=exp_avg.device)
+        v = torch.empty_like(m)
+        _lib.check(_lib.lib().ddcn_adamw_moments(_lib.ptr(exp_avg), _lib.ptr(exp_avg_sq), _lib.ptr(exp_avg_scale),
+                                                 _lib.ptr(exp_avg_sq_scale), _lib.ptr(m), _lib.ptr(v), n,
+                                                 _lib.current_stream(exp_avg.device)))
+    return m, v
+
+
+class _Arena:
+    """The moments of one parameter group's tensors of one type on one GPU."""
+
+    def __init__(self, params, bits):
+        self.key = self.key_of(params)
+        dev, n = params[0].device, adamw_arena(params)
+        zeros = lambda k, t: torch.zeros(k, dtype=t, device=dev)                                  # noqa: E731
+        self.exp_avg = zeros(n, torch.float32 if bits == 32 else torch.int8)
+        self.exp_avg_sq = zeros(n, torch.float32 if bits == 32 else torch.uint8)
+        self.scales = {} if bits == 32 else dict(exp_avg_scale=zeros(n // BLOCK, torch.float32),
+                                                 exp_avg_sq_scale=zeros(n // BLOCK, torch.float32))
+
+    @staticmethod
+    def key_of(params):
+        return tuple(map(id, params)), tuple(map(_Tensor.numel, params))
+
+    def views(self, params):
+        """For each parameter: its part of the arena, under the names of the state dict."""
+        start = 0
+        for p in params:
+            n = p.numel()
+            end = start + -(-n // BLOCK) * BLOCK
+            state = dict(exp_avg=self.exp_avg[start:start + n].view(p.shape),
+                         exp_avg_sq=self.exp_avg_sq[start:start + n].view(p.shape))
+            state.update({k: t[start // BLOCK:end // BLOCK] for k, t in self.scales.items()})
+            yield state
+            start = end
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's interface over `adamw_step`.
+
+    bits=32 or 8: how the moments are held.  max_norm: clip all gradients by their global norm first (the last norm is
+    kept in `last_grad_norm`, a scalar on the GPU); a step whose norm is not finite changes no parameter and no moment,
+    though its step number counts.  seed: of the rounding of 8-bit moments; the same seed repeats a run.
+    Parameters of one group may have different types (one arena each); all live on one GPU."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, max_norm=None, seed=0):
+        if bits not in (32, 8):
+            raise ValueError("moments of %r bits: 32 or 8" % (bits,))
+        if not lr >= 0 or not eps >= 0 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError("lr %r, betas %r, eps %r, weight_decay %r" % (lr, betas, eps, weight_decay))
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError("max_norm %r: above 0, or None" % (max_norm,))
+        self.bits, self.max_norm, self.seed, self.last_grad_norm = bits, max_norm, int(seed), None
+        self._arenas = {}
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def _sets(self, g):
+        """(dtype, parameters) of group number g, in the order of its first parameter of each type."""
+        sets = {}
+        for p in self.param_groups[g]["params"]:
+            sets.setdefault(p.dtype, []).append(p)
+        return sets.items()
+
+    def _arena(self, g, dtype, params):
+        arena = self._arenas.get((g, dtype))
+        if arena is not None and arena.key == _Arena.key_of(params):
+            return arena
+        if arena is not None or any(p in self.state for p in params):
+            raise RuntimeError("ddcn: the parameters of a group (or their types or sizes) changed after its first step")
+        arena = self._arenas[g, dtype] = _Arena(params, self.bits)
+        for p, state in zip(params, arena.views(params)):
+            self.state[p] = dict(step=0, **state)
+        return arena
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        sets = [(g, dtype, params) for g in range(len(self.param_groups)) for dtype, params in self._sets(g)]
+        grads = [[p.grad for p in params] for _, _, params in sets]
+        every = [x for l in grads for x in l if x is not None]
+        if not every:
+            return loss
+        norm = self.last_grad_norm = grad_norm(every) if self.max_norm is not None else None
+        for number, ((g, dtype, params), gs) in enumerate(zip(sets, grads)):
+            if all(x is None for x in gs):
+                continue
+            group, arena, state = self.param_groups[g], self._arena(g, dtype, params), self.state
+            steps = [state[p]["step"] + (x is not None) for p, x in zip(params, gs)]
+            same = steps[0] if steps.count(steps[0]) == len(steps) else None
+            # a seed for every step and arena; step numbers of one arena only grow
+            seed = self.seed + 0x10001 * number + 0x3779B1 * max(steps)
+            adamw_step(params, gs, arena.exp_avg, arena.exp_avg_sq, same or [max(s, 1) for s in steps], group["lr"],
+                       group["betas"], group["eps"], group["weight_decay"], seed=seed, grad_norm=norm,
+                       max_norm=self.max_norm, **arena.scales)
+            for p, s in zip(params, steps):
+                state[p]["step"] = s
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but moments keep their types (torch would cast them to the parameter's) and are copied into the
+        arenas.  A state of another number of bits is refused."""
+        saved = state_dict["state"]
+        super().load_state_dict(dict(state_dict, state={}))
+        self._arenas.clear()
+        self.state.clear()
+        order = {}
+        for group, old in zip(self.param_groups, state_dict["param_groups"]):
+            order.update(zip(group["params"], old["params"]))
+        for g in range(len(self.param_groups)):
+            for dtype, params in self._sets(g):
+                if not any(order[p] in saved for p in params):
+                    continue
+                self._arena(g, dtype, params)
+                for p in params:
+                    mine, theirs = self.state[p], saved.get(order[p])
+                    if theirs is None:
+                        continue
+                    if set(theirs) != set(mine):
+                        raise ValueError("the state dict holds %s, this optimizer %s" % (sorted(theirs), sorted(mine)))
+                    for k, t in theirs.items():
+                        if k == "step":
+                            mine[k] = int(t)
+                        elif t.dtype != mine[k].dtype or t.shape != mine[k].shape:
+                            raise ValueError("%s of the state dict is %s %s, not %s %s" % (
+                                k, t.dtype, tuple(t.shape), mine[k].dtype, tuple(mine[k].shape)))
+                        else:
+                            mine[k].copy_(t)
+
+    def __deepcopy__(self, memo):
+        new = type(self)(copy.deepcopy(self.param_groups, memo), bits=self.bits, max_norm=self.max_norm, seed=self.seed)
+        new.load_state_dict(self.state_dict())
+        return new

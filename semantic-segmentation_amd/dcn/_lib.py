@@ -28,10 +28,29 @@ class RoiGeom(ctypes.Structure):
                  "trans_channels", "no_trans")] + [("spatial_scale", ctypes.c_float), ("trans_std", ctypes.c_float)]
 
 
+class AdamwHyper(ctypes.Structure):
+    """struct ddcn_adamw_hyper (include/ddcn_hip.h)."""
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + \
+        [("step", ctypes.c_int), ("dtype", ctypes.c_int), ("bits", ctypes.c_int), ("seed", ctypes.c_uint)]
+
+
+class Int8Geom(ctypes.Structure):
+    """struct ddcn_int8_geom (include/ddcn_hip.h)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("images", "rows", "cols", "k", "channels", "nchw", "dtype", "out_dtype",
+                                            "relu")] + \
+        [(n, ctypes.c_longlong) for n in ("si", "sh", "sw", "sk", "ldw")]
+
+
+# enum of element types (include/ddcn_hip.h)
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
 _P = ctypes.c_void_p
 _G = ctypes.POINTER(Geom)
 _RG = ctypes.POINTER(RoiGeom)
 _SZ = ctypes.c_size_t
+_HY = ctypes.POINTER(AdamwHyper)
+_IG = ctypes.POINTER(Int8Geom)
+_LL = ctypes.c_longlong
 
 # name -> argtypes; every entry returns int unless listed in _RESTYPES
 PROTOTYPES = {
@@ -95,6 +114,14 @@ PROTOTYPES = {
     "ddcn_deform_psroi_pool_backward_f32": [_P, _P, _P, _P, _P, _P, _P, _RG, _P],
     "ddcn_deform_psroi_pool_forward_f64": [_P, _P, _P, _P, _P, _RG, _P],
     "ddcn_deform_psroi_pool_backward_f64": [_P, _P, _P, _P, _P, _P, _P, _RG, _P],
+    "ddcn_adamw_arena": [ctypes.c_int, _P],
+    "ddcn_adamw_step": [ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, _HY, _P],
+    "ddcn_adamw_moments": [_P, _P, _P, _P, _P, _P, _LL, _P],
+    "ddcn_grad_norm_workspace_bytes": [ctypes.c_int, _P],
+    "ddcn_grad_norm": [ctypes.c_int, _P, _P, _P, _P, _P, _SZ, _P],
+    "ddcn_int8_workspace_bytes": [_IG],
+    "ddcn_int8_product": [_P, _P, _P, _P, _P, _P, _SZ, _IG, _P],
+    "ddcn_int8_quantize": [_P, _P, _LL, _P, _IG, _P],
 }
 _RESTYPES = {
     "ddcn_strerror": ctypes.c_char_p,
@@ -107,6 +134,9 @@ _RESTYPES = {
     "ddcn_gemm_gcol_16_workspace_bytes": _SZ,
     "ddcn_gweight_16_workspace_bytes": _SZ,
     "ddcn_workspace_bytes_f64": _SZ,
+    "ddcn_adamw_arena": ctypes.c_longlong,
+    "ddcn_grad_norm_workspace_bytes": _SZ,
+    "ddcn_int8_workspace_bytes": _SZ,
 }
 
 _lib = None

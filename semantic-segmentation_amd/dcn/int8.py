@@ -1,0 +1,215 @@
+"""Linear layers and 1x1 convolutions in 8-bit integers at inference: y = s_token s_channel sum q w (+ bias, ReLU).
+
+Not in the reference; they stand beside the 16-bit inference of the deformable convolutions (deform_conv.py) and take
+over the layers around them: a bottleneck's 1x1 convolutions, the depth branch, the fc layers of deformable RoI pooling
+(`callers.int8_inference` converts a model).  Weights are rounded once, with one scale per output channel
+(`quantize_int8`); every token -- a RoI, a pixel -- is rounded on the way in, with a scale of its own.  The sums are exact.
+A token that holds a NaN or an infinity gives NaN in all of its outputs.  Kernels: csrc/ddcn_int8.hip; the arithmetic is
+written down in include/ddcn_hip.h.  CPU tensors raise NotImplementedError, tensors that require grad a RuntimeError.
+"""
+import torch
+import torch.nn as nn
+
+from . import _lib
+
+
+def _check_input(name, t):
+    if not t.is_cuda:
+        raise NotImplementedError
+    if t.dtype not in _lib.ELEMENT_TYPES:
+        raise RuntimeError("ddcn: %s of %s is not supported (float32, float16, bfloat16)" % (name, t.dtype))
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise RuntimeError("ddcn: the 8-bit layers have no backward pass: call them under torch.no_grad(), or detach %s"
+                           % name)
+
+
+def _check_weight(x, weight_q, weight_scale, bias, k):
+    """-> (channels, float32 bias)"""
+    for name, t in (("weight_q", weight_q), ("weight_scale", weight_scale), ("bias", bias)):
+        if t is not None and not t.is_cuda:
+            raise NotImplementedError
+        if t is not None and t.device != x.device:
+            raise RuntimeError("ddcn: %s is on %s but the input is on %s" % (name, t.device, x.device))
+    if weight_q.dtype != torch.int8 or weight_q.dim() != 2 or weight_q.shape[1] != k:
+        raise RuntimeError("ddcn: weight_q has to be int8 [channels, %d], got %s %s" % (k, weight_q.dtype, tuple(weight_q.shape)))
+    n = weight_q.shape[0]
+    if weight_scale.dtype != torch.float32 or weight_scale.shape != (n,):
+        raise RuntimeError("ddcn: weight_scale has to be float32 [%d], got %s %s" % (n, weight_scale.dtype, tuple(weight_scale.shape)))
+    if bias is not None:
+        if bias.dtype not in _lib.ELEMENT_TYPES or bias.shape != (n,):
+            raise RuntimeError("ddcn: bias has to be floating point [%d], got %s %s" % (n, bias.dtype, tuple(bias.shape)))
+        _check_input("bias", bias)
+        bias = bias.detach().float().contiguous()
+    return n, bias
+
+
+def _weight_rows(weight_q):
+    """The weights with contiguous values in a row, and the rows' stride in bytes."""
+    if weight_q.stride(1) != 1 and weight_q.shape[1] > 1 or weight_q.shape[0] > 1 and weight_q.stride(0) < weight_q.shape[1]:
+        weight_q = weight_q.contiguous()
+    return weight_q, max(weight_q.stride(0), weight_q.shape[1])
+
+
+def _product(x, y, weight_q, weight_scale, bias, geom):
+    L = _lib.lib()
+    nbytes = L.ddcn_int8_workspace_bytes(geom)
+    with torch.cuda.device(x.device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.check(L.ddcn_int8_product(_lib.ptr(x), _lib.ptr(weight_q), _lib.ptr(weight_scale), _lib.ptr(bias),
+                                       _lib.ptr(y), _lib.ptr(ws), nbytes, geom, _lib.current_stream(x.device)))
+    return y
+
+
+def _out_dtype(x, out_dtype):
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _lib.ELEMENT_TYPES:
+        raise RuntimeError("ddcn: output of %s is not supported (float32, float16, bfloat16)" % out_dtype)
+    return out_dtype
+
+
+def quantize_int8(x):
+    """(q, scale) of the rows of x [rows, k]: int8 [rows, k] and float32 [rows], x ~ q * scale[:, None].  This is the
+    rounding of the tokens of `int8_linear`, and the one to lay a weight [channels, k] out with."""
+    _check_input("x", x)
+    if x.dim() != 2:
+        raise RuntimeError("ddcn: 2D tensor expected but got: %d" % x.dim())
+    rows, k = x.shape
+    if k > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    q = torch.empty((rows, k), dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    g = _lib.Int8Geom(1, rows, 1, k, 1, 0, _lib.ELEMENT_TYPES[x.dtype], 0, 0, 0, x.stride(0), 0, 1, k)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().ddcn_int8_quantize(_lib.ptr(x), _lib.ptr(q), k, _lib.ptr(scale), g,
+                                                 _lib.current_stream(x.device)))
+    return q, scale
+
+
+def int8_linear(input, weight_q, weight_scale, bias=None, relu=False, out_dtype=None):
+    """input [..., k] (float32, float16 or bfloat16), weight_q int8 [channels, k], weight_scale float32 [channels],
+    bias [channels] -> [..., channels] in `out_dtype` (the input's).  Rows of input may be strided."""
+    _check_input("input", input)
+    if input.dim() < 1:
+        raise RuntimeError("ddcn: input has no dimension")
+    k = input.shape[-1]
+    n, bias = _check_weight(input, weight_q, weight_scale, bias, k)
+    dtype = _out_dtype(input, out_dtype)
+    x = input.detach().reshape(-1, k) if k else input
+    y = torch.empty(tuple(input.shape[:-1]) + (n,), dtype=dtype, device=input.device)
+    if not y.numel():
+        return y
+    weight_q, ldw = _weight_rows(weight_q)
+    g = _lib.Int8Geom(1, x.shape[0], 1, k, n, 0, _lib.ELEMENT_TYPES[x.dtype], _lib.ELEMENT_TYPES[dtype], int(relu), 0,
+                      x.stride(0), 0, 1 if k == 1 else x.stride(1), ldw)
+    return _product(x, y, weight_q, weight_scale.contiguous(), bias, g)
+
+
+def int8_conv1x1(input, weight_q, weight_scale, bias=None, stride=1, relu=False, out_dtype=None):
+    """1x1 convolution without padding: input [n, c, h, w] (any strides), weight_q int8 [channels, c] ->
+    [n, channels, ceil(h / stride), ceil(w / stride)], in channels-last memory where the input is."""
+    _check_input("input", input)
+    if input.dim() != 4:
+        raise RuntimeError("4D input tensor expected but got: %d" % input.dim())
+    if int(stride) != stride or stride < 1:
+        raise RuntimeError("stride should be greater than zero, but got %r" % (stride,))
+    stride = int(stride)
+    images, c, h, w = input.shape
+    n, bias = _check_weight(input, weight_q, weight_scale, bias, c)
+    dtype = _out_dtype(input, out_dtype)
+    ho, wo = -(-h // stride), -(-w // stride)
+    last = c > 1 and input.stride(1) == 1
+    y = torch.empty((images, n, ho, wo), dtype=dtype, device=input.device,
+                    memory_format=torch.channels_last if last else torch.contiguous_format)
+    if not y.numel():
+        return y
+    x = input.detach()
+    si, sk, sh, sw = x.stride()
+    weight_q, ldw = _weight_rows(weight_q)
+    g = _lib.Int8Geom(images, ho, wo, c, n, 0 if last else 1, _lib.ELEMENT_TYPES[x.dtype], _lib.ELEMENT_TYPES[dtype],
+                      int(relu), si, sh * stride, sw * stride, sk, ldw)
+    return _product(x, y, weight_q, weight_scale.contiguous(), bias, g)
+
+
+class _Int8Layer(nn.Module):
+    """Weights in int8 with their scales, as buffers; no parameters."""
+
+    def __init__(self, channels, k, bias):
+        super().__init__()
+        self.register_buffer("weight_q", torch.zeros((channels, k), dtype=torch.int8))
+        self.register_buffer("weight_scale", torch.ones(channels, dtype=torch.float32))
+        self.register_buffer("bias", torch.zeros(channels, dtype=torch.float32) if bias else None)
+
+    def _apply(self, fn, recurse=True):
+        # .half() / .bfloat16() move a model to 16-bit activations: scales and bias stay float32
+        super()._apply(fn, recurse)
+        for name in ("weight_scale", "bias"):
+            t = getattr(self, name)
+            if t is not None and t.dtype != torch.float32:
+                setattr(self, name, t.float())
+        return self
+
+    @torch.no_grad()
+    def _fill(self, weight, bias):
+        q, scale = quantize_int8(weight.detach())
+        self.weight_q, self.weight_scale = q, scale
+        if bias is not None:
+            self.bias = bias.detach().float().clone()
+        return self
+
+
+class Int8Linear(_Int8Layer):
+    """nn.Linear at inference, in 8 bits; `relu` applies one behind it."""
+
+    def __init__(self, in_features, out_features, bias=True, relu=False):
+        super().__init__(out_features, in_features, bias)
+        self.in_features, self.out_features, self.relu = in_features, out_features, relu
+
+    @classmethod
+    def from_float(cls, layer, relu=False):
+        """From an nn.Linear on the GPU."""
+        new = cls(layer.in_features, layer.out_features, layer.bias is not None, relu)
+        return new._fill(layer.weight, layer.bias)
+
+    def forward(self, x):
+        return int8_linear(x, self.weight_q, self.weight_scale, self.bias, self.relu)
+
+    def extra_repr(self):
+        return "in_features=%d, out_features=%d, bias=%s, relu=%s" % (self.in_features, self.out_features,
+                                                                      self.bias is not None, self.relu)
+
+
+class Int8Conv1x1(_Int8Layer):
+    """nn.Conv2d(kernel_size=1) at inference, in 8 bits, with the batch norm behind it folded in; `relu` applies one."""
+
+    def __init__(self, in_channels, out_channels, stride=1, bias=True, relu=False):
+        super().__init__(out_channels, in_channels, bias)
+        self.in_channels, self.out_channels, self.stride, self.relu = in_channels, out_channels, stride, relu
+
+    @classmethod
+    def from_float(cls, conv, norm=None, relu=False):
+        """From an nn.Conv2d on the GPU (1x1, no padding, one group) and, optionally, the nn.BatchNorm2d behind it: its
+        running statistics and affine become part of the weights (before they are rounded) and of the bias."""
+        if tuple(conv.kernel_size) != (1, 1) or conv.groups != 1 or conv.stride[0] != conv.stride[1] or \
+                conv.padding not in ((0, 0), "valid"):
+            raise ValueError("not a 1x1 convolution without padding and groups: %r" % (conv,))
+        weight, bias = conv.weight.detach().float().flatten(1), conv.bias
+        if norm is not None:
+            if norm.running_mean is None:
+                raise ValueError("the norm layer keeps no running statistics: %r" % (norm,))
+            factor = torch.rsqrt(norm.running_var.float() + norm.eps)
+            if norm.weight is not None:
+                factor = factor * norm.weight.detach().float()
+            shift = -norm.running_mean.float() if bias is None else bias.detach().float() - norm.running_mean.float()
+            bias = shift * factor
+            if norm.bias is not None:
+                bias = bias + norm.bias.detach().float()
+            weight = weight * factor[:, None]
+        new = cls(conv.in_channels, conv.out_channels, conv.stride[0], bias is not None, relu)
+        return new._fill(weight, bias)
+
+    def forward(self, x):
+        return int8_conv1x1(x, self.weight_q, self.weight_scale, self.bias, self.stride, self.relu)
+
+    def extra_repr(self):
+        return "%d, %d, stride=%d, bias=%s, relu=%s" % (self.in_channels, self.out_channels, self.stride,
+                                                        self.bias is not None, self.relu)

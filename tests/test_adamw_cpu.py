@@ -1,0 +1,103 @@
+"""CPU: what the AdamW entry points refuse before anything is launched, the arena's layout, and the 8-bit codes'
+arithmetic (in the numpy restatement that the GPU tests compare with)."""
+import ctypes
+import importlib
+from array import array
+
+import numpy as np
+import pytest
+import torch
+
+import adamw_ref as ref
+from conftest import load_pkg
+
+load_pkg()
+callers = importlib.import_module("semantic-segmentation_amd.callers")
+_lib = importlib.import_module("semantic-segmentation_amd.dcn._lib")
+
+
+def _a(kind, values):
+    a = array(kind, values)
+    return a, ctypes.c_void_p(a.buffer_info()[0])
+
+
+def test_arena_starts_tensors_on_blocks():
+    assert callers.adamw_arena([torch.zeros(n) for n in (1, 256, 257, 0, 3)]) == 256 + 256 + 512 + 0 + 256
+    assert callers.adamw_arena([]) == 0
+    keep, p = _a("q", [-1])
+    assert _lib.lib().ddcn_adamw_arena(1, p) == -2
+
+
+def _step(**kw):
+    """Return code of a step over one tensor that must fail (or be empty) before it launches anything."""
+    d = dict(count=1, p=4096, g=8192, n=256, m=16384, v=32768, sm=64, sv=64, norm=None, lr=1e-3, b1=0.9, b2=0.999,
+             eps=1e-8, wd=0.01, max_norm=1.0, step=1, dtype=0, bits=32)
+    d.update(kw)
+    (k1, p), (k2, g), (k3, n) = _a("Q", [d["p"]]), _a("Q", [d["g"]]), _a("q", [d["n"]])
+    h = _lib.AdamwHyper(d["lr"], d["b1"], d["b2"], d["eps"], d["wd"], d["max_norm"], d["step"], d["dtype"], d["bits"], 0)
+    return _lib.lib().ddcn_adamw_step(d["count"], p, g, n, None, d["m"], d["v"], d["sm"], d["sv"], d["norm"], h, None)
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(count=-1), -1), (dict(n=-5), -2), (dict(m=None), -1), (dict(bits=16), -5),
+                                   (dict(bits=8, sm=None), -1), (dict(dtype=3), -5), (dict(m=16392), -1),
+                                   (dict(p=4098), -1), (dict(g=8193, dtype=1), -1), (dict(p=0), -1), (dict(step=0), -1),
+                                   (dict(b1=1.0), -1), (dict(lr=float("nan")), -1), (dict(eps=-1.0), -1),
+                                   (dict(norm=64, max_norm=0.0), -1), (dict(n=0), 0), (dict(count=0), 0)])
+def test_step_refuses_bad_arguments(kw, rc):
+    assert _step(**kw) == rc, _lib.lib().ddcn_last_error()
+
+
+def test_norm_and_moments_refuse_bad_arguments():
+    L = _lib.lib()
+    (k1, g), (k2, n), (k3, t) = _a("Q", [4096]), _a("q", [100]), _a("i", [0])
+    need = L.ddcn_grad_norm_workspace_bytes(1, n)
+    assert need == 256
+    call = lambda g, n, t, out=64, ws=256, size=need: L.ddcn_grad_norm(1, g, n, t, out, ws, size, None)   # noqa: E731
+    assert call(g, n, t, size=need - 1) == -3
+    assert call(g, n, t, out=None) == -1 and call(g, n, t, ws=8) == -1
+    k4, bad_type = _a("i", [7])
+    k5, odd = _a("Q", [4098])
+    k6, null = _a("Q", [0])
+    assert call(g, n, bad_type) == -5 and call(odd, n, t) == -1 and call(null, n, t) == -1
+    assert L.ddcn_adamw_moments(64, 64, 64, 64, 64, 64, 100, None) == -2
+    assert L.ddcn_adamw_moments(64, 64, 64, 64, 64, 72, 256, None) == -1
+    assert L.ddcn_adamw_moments(None, 64, 64, 64, 64, 64, 256, None) == -1
+
+
+def test_cpu_tensors_raise_not_implemented():
+    p, g = [torch.zeros(4)], [torch.zeros(4)]
+    with pytest.raises(NotImplementedError):
+        callers.grad_norm(g)
+    with pytest.raises(NotImplementedError):
+        callers.adamw_step(p, g, torch.zeros(256), torch.zeros(256), 1, 1e-3)
+    with pytest.raises(NotImplementedError):
+        callers.adamw_moments(torch.zeros(256, dtype=torch.int8), torch.zeros(256, dtype=torch.uint8), torch.zeros(1), torch.zeros(1))
+
+
+def test_optimizer_refuses_bad_settings():
+    p = [torch.nn.Parameter(torch.zeros(4))]
+    for kw in (dict(bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(max_norm=0.0)):
+        with pytest.raises(ValueError):
+            callers.AdamW(p, **kw)
+    callers.AdamW(p).step()      # no gradients: nothing happens, on a CPU model too
+
+
+def test_codes_are_unbiased_and_ordered():
+    """Mean of the decoded roots over many places against the value: u is uniform on 2^16 points, so that the mean of
+    floor(x + u) over N draws is x within 5 sigma of a Bernoulli sum, 5 * 0.5 / sqrt(N)."""
+    n = 1 << 16
+    um, uv = ref.noise(np.arange(n), 7)
+    for x in (0.25, 3.4, 100.9):
+        q = np.floor(np.float32(x) + um)
+        assert abs(q.mean() - x) < 2.5 / np.sqrt(n) + 2.0 ** -16
+        q = np.floor(np.float32(x) + uv)
+        assert abs(q.mean() - x) < 2.5 / np.sqrt(n) + 2.0 ** -16
+    # the largest value of a block is held exactly up to the two roundings of its scale
+    q, s = ref.encode(np.array([1.0, 0.5, 0.0], np.float32), np.zeros(3, np.float32), 127)
+    assert q[0] == 127 and q[2] == 0 and abs(float(ref.decode_m(q, s)[0]) - 1) < 2 ** -22
+    assert 89 <= q[1] <= 90
+
+
+def test_another_seed_gives_other_numbers():
+    a, b = ref.noise(np.arange(4096), 1), ref.noise(np.arange(4096), 2)
+    assert (a[0] != b[0]).mean() > 0.99 and (a[1] != b[1]).mean() > 0.99
