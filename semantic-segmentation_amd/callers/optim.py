@@ -35,42 +35,43 @@ def _one_device(tensors, name):
 
 
 def _check_layout(tensors, name):
-    for t in tensors:
-        if t.layout is not torch.strided:
-            raise RuntimeError("ddcn: %s must be dense tensors, got %s" % (name, t.layout))
+    # (a sparse tensor raises a RuntimeError of torch's own here)
     if not all(map(_Tensor.is_contiguous, tensors)):
         raise RuntimeError("ddcn: %s tensors have to be contiguous" % name)
 
 
-def adamw_arena(params):
-    """Elements of the arena that holds one moment of `params`."""
-    numels = array("q", map(_Tensor.numel, params))
+def _arena_of(numels):
     n = _lib.lib().ddcn_adamw_arena(len(numels), _address(numels))
     if n < 0:
         _lib.check(n)
     return n
 
 
+def adamw_arena(params):
+    """Elements of the arena that holds one moment of `params`."""
+    return _arena_of(array("q", map(_Tensor.numel, params)))
+
+
 def grad_norm(grads):
     """sqrt of the sum of squares over all `grads` (entries may be None), a float32 scalar on their GPU: summed in
     float64 in a fixed order, so that it is the same at every call.  Types may be mixed."""
-    grads = [g.detach() for g in grads if g is not None]
+    grads = [g for g in grads if g is not None]
     if not grads:
         raise RuntimeError("ddcn: grad_norm needs at least one gradient")
     dev = _one_device(grads, "gradients")
     _check_layout(grads, "gradient")
     try:
-        dtypes = array("i", [_lib.ELEMENT_TYPES[g.dtype] for g in grads])
+        dtypes = array("i", map(_lib.ELEMENT_TYPES.__getitem__, map(_dtype_of, grads)))
     except KeyError as e:
         raise RuntimeError("ddcn: %s gradients are not supported (float32, float16, bfloat16)" % e) from None
     pointers, numels = array("Q", map(_Tensor.data_ptr, grads)), array("q", map(_Tensor.numel, grads))
     L = _lib.lib()
     nbytes = L.ddcn_grad_norm_workspace_bytes(len(grads), _address(numels))
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device)
         out = torch.empty((), dtype=torch.float32, device=grads[0].device)
         _lib.check(L.ddcn_grad_norm(len(grads), _address(pointers), _address(numels), _address(dtypes), _lib.ptr(out),
-                                    _lib.ptr(ws), nbytes, _lib.current_stream(grads[0].device)))
+                                    _lib.ptr(ws), nbytes, _lib.stream_of(dev)))
     return out
 
 
@@ -104,11 +105,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
     if not params:
         return
     dtype = params[0].dtype
-    if any(g is None for g in grads):
-        given = [g for g in grads if g is not None]
-        mine = [p for p, g in zip(params, grads) if g is not None]
-    else:
-        given, mine = grads, params
+    given = [g for g in grads if g is not None]
+    mine = params if len(given) == len(grads) else [p for p, g in zip(params, grads) if g is not None]
     dev = _one_device(params + given + ([grad_norm] if grad_norm is not None else []), "parameters and gradients")
     if dtype not in _lib.ELEMENT_TYPES:
         raise RuntimeError("ddcn: %s parameters are not supported (float32, float16, bfloat16)" % dtype)
@@ -117,14 +115,15 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
     _check_layout(params, "parameter")
     _check_layout(given, "gradient")
     numels = array("q", map(_Tensor.numel, params))
-    if list(map(_Tensor.numel, given)) != (numels.tolist() if given is grads else list(map(_Tensor.numel, mine))):
+    if array("q", map(_Tensor.numel, given)) != (numels if mine is params else array("q", map(_Tensor.numel, mine))):
         raise RuntimeError("ddcn: a gradient has another number of elements than its parameter")
     pointers = array("Q", map(_Tensor.data_ptr, params))
-    starts = [a for a, n in zip(pointers, numels) if n]
-    if len(set(starts)) != len(starts):
-        raise RuntimeError("ddcn: a parameter is listed twice")
+    if len(set(pointers)) != len(pointers):            # (empty tensors may share an address)
+        starts = [a for a, n in zip(pointers, numels) if n]
+        if len(set(starts)) != len(starts):
+            raise RuntimeError("ddcn: a parameter is listed twice")
     L = _lib.lib()
-    arena = adamw_arena(params)
+    arena = _arena_of(numels)
     bits = 8 if exp_avg.dtype == torch.int8 else 32
     _check_state("exp_avg", exp_avg, torch.int8 if bits == 8 else torch.float32, arena, dev)
     _check_state("exp_avg_sq", exp_avg_sq, torch.uint8 if bits == 8 else torch.float32, arena, dev)
@@ -149,12 +148,15 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
                            "the learning rate and the seed of the capture")
     hyper = _lib.AdamwHyper(lr, betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, step,
                             _lib.ELEMENT_TYPES[dtype], bits, int(seed) & 0xFFFFFFFF)
-    gradients = array("Q", [0 if g is None else g.data_ptr() for g in grads])
-    with torch.cuda.device(dev):
+    if mine is params:
+        gradients = array("Q", map(_Tensor.data_ptr, grads))
+    else:
+        gradients = array("Q", [0 if g is None else g.data_ptr() for g in grads])
+    with _lib.on_device(dev):
         _lib.check(L.ddcn_adamw_step(len(params), _address(pointers), _address(gradients), _address(numels),
                                      None if steps is None else _address(steps), _lib.ptr(exp_avg),
                                      _lib.ptr(exp_avg_sq), _lib.ptr(exp_avg_scale), _lib.ptr(exp_avg_sq_scale),
-                                     _lib.ptr(grad_norm), hyper, _lib.current_stream(params[0].device)))
+                                     _lib.ptr(grad_norm), hyper, _lib.stream_of(dev)))
     # the kernels write behind autograd's back: a backward pass that saved one of these must notice
     torch.autograd.graph.increment_version(mine + [exp_avg, exp_avg_sq] +
                                            ([exp_avg_scale, exp_avg_sq_scale] if bits == 8 else []))
@@ -171,12 +173,12 @@ def adamw_moments(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
     _check_state("exp_avg_sq", exp_avg_sq, torch.uint8, n, dev)
     _check_state("exp_avg_scale", exp_avg_scale, torch.float32, n // BLOCK, dev)
     _check_state("exp_avg_sq_scale", exp_avg_sq_scale, torch.float32, n // BLOCK, dev)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         m = torch.empty(n, dtype=torch.float32, device=exp_avg.device)
         v = torch.empty_like(m)
         _lib.check(_lib.lib().ddcn_adamw_moments(_lib.ptr(exp_avg), _lib.ptr(exp_avg_sq), _lib.ptr(exp_avg_scale),
                                                  _lib.ptr(exp_avg_sq_scale), _lib.ptr(m), _lib.ptr(v), n,
-                                                 _lib.current_stream(exp_avg.device)))
+                                                 _lib.stream_of(dev)))
     return m, v
 
 

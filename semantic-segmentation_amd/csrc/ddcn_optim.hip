@@ -2,9 +2,10 @@
 // The formulas stand in include/ddcn_hip.h; they are evaluated here operation by operation, each rounded to fp32 (no
 // fused multiply-adds in the moments), so that a code does not depend on how a compiler contracts an expression.
 //
-// The tensors of a launch travel as kernel arguments (up to 96 of them): no device table to keep, nothing that a later
-// launch or another stream could overwrite.  One wave handles 256 consecutive elements of a tensor, four per lane -- in
-// 8 bits a block of one pair of scales, whose maxima are one wave reduction.
+// The tensors of a launch travel as kernel arguments (up to 160 of them): no device table to keep, nothing that a later
+// launch or another stream could overwrite.  One wave handles blocks of 256 consecutive elements of the arena, four per
+// lane, whichever tensors they belong to -- in 8 bits a block is what one pair of scales stands for, and their maxima are
+// one wave reduction.
 #include <math.h>
 
 #include "ddcn_elem.h"
@@ -12,151 +13,279 @@
 namespace ddcn {
 namespace {
 
-constexpr int kBlock = 256;                     // elements per pair of scales, and per wave
+constexpr int kBlock = 256;             // elements per pair of scales, and per wave and turn
 constexpr int kWaves = 4;
-constexpr int kBlocksPerWave = 4;
-constexpr int kChunkBlocks = kWaves * kBlocksPerWave;   // blocks of a workgroup
 
-struct AdamwTensor {
-    void *p;
-    const void *g;
-    long long n;
-    unsigned block0;       // first 256-element block in the arena
-    unsigned chunk0;       // first workgroup of the launch
-    float step_size;       // lr / (1 - beta1^t)
-    float rsqrt_bc2;       // 1 / sqrt(1 - beta2^t)
-};
-constexpr int kMaxTensors = 96;
+constexpr int kMaxTensors = 160;
 struct AdamwArgs {
-    AdamwTensor t[kMaxTensors];
+    // tensor j of the launch covers the arena's blocks block0[j] .. block0[j+1]-1 (relative to `first`); n[j] elements.
+    // A null gradient: its blocks are left alone.
+    void *p[kMaxTensors];
+    const void *g[kMaxTensors];
+    unsigned block0[kMaxTensors];
+    unsigned n[kMaxTensors];
     void *m, *v;
     float *sm, *sv;
     const float *norm;
+    long long first;       // block of the arena that the launch begins with
+    unsigned blocks;       // of the launch
     float b1, ob1, b2, ob2, eps, decay, max_norm;
+    float step_size;       // lr / (1 - beta1^t)
+    float rsqrt_bc2;       // 1 / sqrt(1 - beta2^t)
     unsigned seed;
     int count;
 };
 static_assert(sizeof(AdamwArgs) <= 4096, "kernel argument segment");
 
-// The last entry whose first workgroup is not behind workgroup b
-template <typename A>
-__device__ __forceinline__ int find_tensor(const A &a, unsigned b)
-{
-    int lo = 0, hi = a.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.t[mid].chunk0 <= b) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
-
 // Largest of non-negative floats over the wave, on their bits: ordered as the numbers are, NaN above infinity, so that
-// one NaN is not lost
+// one NaN is not lost.  Five steps within and across rows of 16 lanes on the DPP network and one row broadcast; lane 63
+// has the result.
 __device__ __forceinline__ unsigned wave_max_bits(unsigned x)
 {
-    for (int d = 32; d; d >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, d));
-    return x;
+#define DDCN_DPP_MAX(ctrl, rows) x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false))
+    DDCN_DPP_MAX(0x111, 0xf);       // row_shr:1
+    DDCN_DPP_MAX(0x112, 0xf);       // row_shr:2
+    DDCN_DPP_MAX(0x114, 0xf);       // row_shr:4
+    DDCN_DPP_MAX(0x118, 0xf);       // row_shr:8
+    DDCN_DPP_MAX(0x142, 0xa);       // row_bcast:15 into rows 1 and 3
+    DDCN_DPP_MAX(0x143, 0xc);       // row_bcast:31 into rows 2 and 3
+#undef DDCN_DPP_MAX
+    return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
 
 // Two 16-bit numbers for an element, from its place in the arena: multiply-xorshift with odd factors (first bits of the
-// golden ratio and of the square roots of 17, 19, 2 and 11)
-__device__ __forceinline__ unsigned noise(unsigned place, unsigned seed)
+// golden ratio and of the square roots of 17, 19, 2 and 11).  `h`: place * golden + seed part
+constexpr unsigned kGolden = 0x9E3779B1u;
+__device__ __forceinline__ unsigned noise(unsigned h)
 {
-    unsigned h = place * 0x9E3779B1u + (seed * 0x1F83D9ABu + 0x5BE0CD19u);
     h = (h ^ (h >> 16)) * 0x6A09E667u;
     h = (h ^ (h >> 15)) * 0x510E527Fu;
     return h ^ (h >> 15);
 }
 
+// Correctly rounded square root for x = 0 or x above 2^-96, where the hardware root (one unit off at most) needs no
+// scaling: the neighbours' residuals decide.  Below, the result may be off by a unit of its own size (under 2^-48).
+__device__ __forceinline__ float sqrt_rn(float x)
+{
+    float s = __builtin_amdgcn_sqrtf(x);
+    const float dn = __uint_as_float(__float_as_uint(s) - 1u), up = __uint_as_float(__float_as_uint(s) + 1u);
+    const float ed = fmaf(-dn, s, x), eu = fmaf(-up, s, x);
+    s = ed <= 0.f ? dn : s;
+    return eu > 0.f ? up : s;
+}
+
 constexpr unsigned kTiny = 0x0D800000u;      // 2^-100
 constexpr unsigned kInf = 0x7F800000u;
 
-// scale of a block with the largest value `bits`, and its reciprocal
-__device__ __forceinline__ void block_scale(unsigned bits, float top2, float &scale, float &inverse)
+struct Place {
+    void *p;
+    const void *g;
+    long long i, at, block;    // element in the tensor (this lane's first), in the arena, block of the arena
+    int live;                  // elements of this lane's four that exist
+    bool wide;                 // all 256 elements exist and both addresses allow wide accesses
+};
+
+// What one lane holds of a block between its loads and its stores
+template <int BITS> struct Held {
+    float p[4], g[4], m[4], v[4];      // m, v: fp32 moments
+    unsigned qm, qv;                   // or their codes and scales
+    float sm, sv;
+};
+
+template <int DT, int BITS> __device__ __forceinline__ void load_block(const AdamwArgs &a, const Place &w, bool wide, Held<BITS> &h)
+{
+    if (wide) {
+        load_four<DT>(w.p, w.i, h.p);
+        load_four<DT>(w.g, w.i, h.g);
+    } else {
+        load_some<DT>(w.p, w.i, w.live, false, h.p);
+        load_some<DT>(w.g, w.i, w.live, false, h.g);
+    }
+    if (BITS == 32) {
+        load_four<DDCN_F32>(a.m, w.at, h.m);
+        load_four<DDCN_F32>(a.v, w.at, h.v);
+    } else {
+        h.qm = *(const unsigned *)((const char *)a.m + w.at);
+        h.qv = *(const unsigned *)((const char *)a.v + w.at);
+        h.sm = a.sm[w.block];
+        h.sv = a.sv[w.block];
+    }
+}
+
+// The four codes of both moments.  EXACT: every root correctly rounded, as the codes are defined.  Otherwise from the
+// hardware's roots: root + u is then off by less than 2^-15 (m: root <= 127, one unit of 2^-17 at the root and half a unit
+// at the sum) and 2^-13 (r: root <= 255, relative 2^-21 from the root of v, the product with the reciprocal, the second
+// root and the sum), so that its floor is the defined one unless it lies that close to a whole number -- `far` says how
+// far the worst of them is from the middle between two.
+template <bool EXACT>
+__device__ __forceinline__ void encode(const float (&m)[4], const float (&v)[4], const float (&r)[4], float im, float iv,
+                                       unsigned h0, unsigned &qm, unsigned &qv, float &far_m, float &far_r)
 {
 #pragma clang fp contract(off)
-    scale = bits < kTiny ? 0.f : bits >= kInf ? __uint_as_float(0x7FC00000u) : __uint_as_float(bits) / top2;
-    inverse = bits < kTiny || bits >= kInf ? 0.f : 1.f / scale;
+    qm = qv = 0;
+    far_m = far_r = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const unsigned u = noise(h0 + (unsigned)e * kGolden);
+        const float tm = fabsf(m[e]) * im, tr = (EXACT ? sqrtf(v[e]) : r[e]) * iv;
+        // fma: the 16-bit number is exact, so that this is the one rounding of root + u
+        const float xm = fmaf((float)(u & 0xFFFFu), 0x1p-16f, EXACT ? sqrt_rn(tm) : __builtin_amdgcn_sqrtf(tm));
+        const float xr = fmaf((float)(u >> 16), 0x1p-16f, EXACT ? sqrt_rn(tr) : __builtin_amdgcn_sqrtf(tr));
+        if (!EXACT) {
+            far_m = fmaxf(far_m, fabsf(__builtin_amdgcn_fractf(xm) - 0.5f));
+            far_r = fmaxf(far_r, fabsf(__builtin_amdgcn_fractf(xr) - 0.5f));
+        }
+        const int q = (int)copysignf(fminf(floorf(xm), 127.f), m[e]);
+        const float k = fmaxf(floorf(xr), v[e] > 0.f ? 1.f : 0.f);     // a code of at least 1 where v > 0
+        qm |= (unsigned)(q & 255) << (8 * e);
+        qv |= (unsigned)fminf(k, 255.f) << (8 * e);
+    }
+}
+
+// Lanes below 32 hold the largest |m| of a block, the others its largest r, as bits: their scales and reciprocals.
+// x / 127^2 and x / 255^2 by the reciprocal and one residual, which is correctly rounded for these two divisors.
+struct Scales {
+    float sm, im, sv, iv;
+};
+__device__ __forceinline__ Scales block_scales(unsigned bits)
+{
+#pragma clang fp contract(off)
+    const bool low = (threadIdx.x & 32) == 0;
+    const float top2 = low ? 16129.f : 65025.f, rec = low ? 1.f / 16129.f : 1.f / 65025.f;
+    const float x = __uint_as_float(bits), q0 = x * rec;
+    const float s = fmaf(fmaf(-q0, top2, x), rec, q0);
+    const float scale = bits < kTiny ? 0.f : bits >= kInf ? __uint_as_float(0x7FC00000u) : s;
+    const float inverse = bits < kTiny || bits >= kInf ? 0.f : 1.f / s;
+    auto lane = [](float f, int l) { return __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(f), l)); };
+    return Scales{lane(scale, 0), lane(inverse, 0), lane(scale, 32), lane(inverse, 32)};
 }
 
 template <int DT, int BITS>
-__global__ __launch_bounds__(64 * kWaves) void adamw_kernel(const AdamwArgs a)
+__device__ __forceinline__ void update_block(const AdamwArgs &a, const Place &w, bool wide, float c, Held<BITS> &h)
 {
 #pragma clang fp contract(off)
+    float m[4], v[4], r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (BITS == 32) {
+            m[e] = h.m[e];
+            v[e] = h.v[e];
+        } else {
+            const float q = (float)(int)(signed char)(h.qm >> (8 * e)), k = (float)((h.qv >> (8 * e)) & 255u);
+            m[e] = h.sm * (q * fabsf(q));                 // q|q| and k k are whole numbers below 2^24
+            const float ro = h.sv * (k * k);
+            v[e] = ro * ro;
+        }
+        const float ge = h.g[e] * c;
+        m[e] = a.b1 * m[e] + a.ob1 * ge;
+        v[e] = a.b2 * v[e] + (a.ob2 * ge) * ge;
+        if (BITS == 8 && !wide && e >= w.live) m[e] = v[e] = 0.f;
+    }
+    // The parameter's own arithmetic may be fused and take the hardware's roots: nothing is decided on its last bits.
+    // Without an eps that hides it, a root of the smallest numbers has to be right.
+    if (a.eps >= 0x1p-40f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = __builtin_amdgcn_sqrtf(v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = sqrtf(v[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        h.p[e] = fmaf(-a.step_size, m[e] * __builtin_amdgcn_rcpf(fmaf(r[e], a.rsqrt_bc2, a.eps)), h.p[e] * a.decay);
+    if (wide) store_four<DT>(w.p, w.i, h.p);
+    else store_some<DT>(w.p, w.i, w.live, false, h.p);
+    if (BITS == 32) {
+        // the arena is padded to whole blocks; what lies behind the tensor's end stays as it was
+        if (wide) {
+            store_four<DDCN_F32>(a.m, w.at, m);
+            store_four<DDCN_F32>(a.v, w.at, v);
+        } else {
+            store_some<DDCN_F32>(a.m, w.at, w.live, true, m);
+            store_some<DDCN_F32>(a.v, w.at, w.live, true, v);
+        }
+        return;
+    }
+    unsigned top_m = 0, top_v = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        top_m = max(top_m, __float_as_uint(m[e]) & 0x7FFFFFFFu);
+        top_v = max(top_v, __float_as_uint(v[e]));         // never negative, nor -0
+    }
+    top_m = wave_max_bits(top_m);
+    top_v = wave_max_bits(top_v) & 0x7FFFFFFFu;
+    constexpr unsigned kSmall = 0x12800000u;               // 2^-90: below, the hardware's roots of v may be off
+    const bool small = top_v < kSmall;
+    const float top_r = small ? sqrtf(__uint_as_float(top_v)) : sqrt_rn(__uint_as_float(top_v));
+    const Scales s = block_scales((threadIdx.x & 32) == 0 ? top_m : __float_as_uint(top_r));
+    unsigned qm, qv;
+    float far_m, far_r;
+    const unsigned h0 = (unsigned)w.at * kGolden + (a.seed * 0x1F83D9ABu + 0x5BE0CD19u);
+    encode<false>(m, v, r, s.im, s.iv, h0, qm, qv, far_m, far_r);
+    if (small || __any(!(far_m < 0.5f - 0x1p-15f) || !(far_r < 0.5f - 0x1p-13f)))
+        encode<true>(m, v, r, s.im, s.iv, h0, qm, qv, far_m, far_r);
+    *(unsigned *)((char *)a.m + w.at) = qm;
+    *(unsigned *)((char *)a.v + w.at) = qv;
+    if ((threadIdx.x & 63) == 0) {
+        a.sm[w.block] = s.sm;
+        a.sv[w.block] = s.sv;
+    }
+}
+
+// U blocks per wave, one after the other in the arena; where all of them are whole, every load is issued before the first
+// result is needed
+template <int DT, int BITS, int U>
+__global__ __launch_bounds__(64 * kWaves) void adamw_kernel(const AdamwArgs a)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // the tensor of a block: how many of the sorted first blocks are not behind it, 64 compared at once
+    unsigned b0[3];
+    for (int i = 0; i < 3; ++i) b0[i] = lane + 64 * i < a.count ? a.block0[min(lane + 64 * i, kMaxTensors - 1)] : 0xFFFFFFFFu;
     float c = 1.f;
     if (a.norm) {
         const float norm = *a.norm;
         if (!isfinite(norm)) return;
         c = fminf(1.f, a.max_norm / (norm + 1e-6f));
     }
-    const int j = find_tensor(a, blockIdx.x);
-    const AdamwTensor &t = a.t[j];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr unsigned kMask = DT == DDCN_F32 ? 15u : 7u;
-    const bool vec_p = ((unsigned long long)t.p & kMask) == 0, vec_g = ((unsigned long long)t.g & kMask) == 0;
-    const long long blocks = (t.n + kBlock - 1) / kBlock;
-    for (int u = 0; u < kBlocksPerWave; ++u) {
-        const long long blk = (long long)(blockIdx.x - t.chunk0) * kChunkBlocks + u * kWaves + wave;
-        if (blk >= blocks) return;
-        const long long i = blk * kBlock + lane * 4;                       // in the tensor
-        const long long at = ((long long)t.block0 + blk) * kBlock + lane * 4;    // in the arena
-        const int live = (int)min(max(t.n - i, 0LL), 4LL);
-        float p[4], g[4], m[4], v[4], r[4];
-        load_some<DT>(t.p, i, live, vec_p, p);
-        load_some<DT>(t.g, i, live, vec_g, g);
-        if (BITS == 32) {
-            load_four<DDCN_F32>(a.m, at, m);
-            load_four<DDCN_F32>(a.v, at, v);
-        } else {
-            const int qm = *(const int *)((const signed char *)a.m + at);
-            const unsigned qv = *(const unsigned *)((const unsigned char *)a.v + at);
-            const float sm = a.sm[t.block0 + blk], sv = a.sv[t.block0 + blk];
-            for (int e = 0; e < 4; ++e) {
-                const int q = (int)(signed char)(qm >> (8 * e)), w = (int)((qv >> (8 * e)) & 255u);
-                m[e] = sm * (float)(q * abs(q));
-                const float ro = sv * (float)(w * w);
-                v[e] = ro * ro;
-            }
-        }
-        unsigned top_m = 0, top_r = 0;
-        for (int e = 0; e < 4; ++e) {
-            const float ge = g[e] * c;
-            m[e] = a.b1 * m[e] + a.ob1 * ge;
-            v[e] = a.b2 * v[e] + (a.ob2 * ge) * ge;
-            r[e] = sqrtf(v[e]);
-            if (BITS == 8 && e >= live) m[e] = r[e] = 0.f;
-            p[e] = p[e] * a.decay - t.step_size * (m[e] / (r[e] * t.rsqrt_bc2 + a.eps));
-            top_m = max(top_m, __float_as_uint(fabsf(m[e])));
-            top_r = max(top_r, __float_as_uint(fabsf(r[e])));
-        }
-        store_some<DT>(t.p, i, live, vec_p, p);
-        if (BITS == 32) {
-            // the arena is padded to whole blocks; what lies behind the tensor's end stays as it was
-            store_some<DDCN_F32>(a.m, at, live, true, m);
-            store_some<DDCN_F32>(a.v, at, live, true, v);
-        } else {
-            float sm, im, sv, iv;
-            block_scale(wave_max_bits(top_m), 127.f * 127.f, sm, im);
-            block_scale(wave_max_bits(top_r), 255.f * 255.f, sv, iv);
-            unsigned qm = 0, qv = 0;
-            for (int e = 0; e < 4; ++e) {
-                const unsigned h = noise((unsigned)(at + e), a.seed);
-                const float um = (float)(h & 0xFFFFu) * 0x1p-16f, uv = (float)(h >> 16) * 0x1p-16f;
-                int q = im > 0.f ? (int)fminf(floorf(sqrtf(fabsf(m[e]) * im) + um), 127.f) : 0;
-                if (m[e] < 0.f) q = -q;
-                int w = iv > 0.f ? (int)fminf(floorf(sqrtf(r[e] * iv) + uv), 255.f) : 0;
-                if (r[e] > 0.f && iv > 0.f) w = max(w, 1);
-                qm |= (unsigned)(q & 255) << (8 * e);
-                qv |= (unsigned)w << (8 * e);
-            }
-            *(unsigned *)((signed char *)a.m + at) = qm;
-            *(unsigned *)((unsigned char *)a.v + at) = qv;
-            if (lane == 0) {
-                a.sm[t.block0 + blk] = sm;
-                a.sv[t.block0 + blk] = sv;
-            }
-        }
+    const unsigned first = (blockIdx.x * kWaves + wave) * U;
+    auto place = [&](unsigned b) {
+        Place w = {};
+        if (b >= a.blocks) return w;
+        int j = -1;
+        for (int i = 0; i < 3; ++i) j += __popcll(__ballot(b0[i] <= b));
+        w.p = a.p[j];
+        w.g = a.g[j];
+        const unsigned begin = (b - a.block0[j]) * kBlock, n = a.n[j];           // n at most 2^31
+        w.i = (long long)begin + lane * 4;
+        w.block = a.first + b;
+        w.at = w.block * kBlock + lane * 4;
+        w.live = (int)max(min((long long)n - w.i, 4LL), 0LL);
+        w.wide = w.g && begin + kBlock <= n && (((unsigned long long)w.p | (unsigned long long)w.g) & kMask) == 0;
+        return w;
+    };
+    Place w[U];
+    bool all = true;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        w[u] = place(first + u);
+        all = all && w[u].wide;
+    }
+    if (all) {
+        Held<BITS> h[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_block<DT, BITS>(a, w[u], true, h[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) update_block<DT, BITS>(a, w[u], true, c, h[u]);
+        return;
+    }
+#pragma unroll 1
+    for (int u = 0; u < U; ++u) {
+        const Place x = place(first + u);
+        if (!x.g) continue;
+        Held<BITS> h;
+        load_block<DT, BITS>(a, x, x.wide, h);
+        update_block<DT, BITS>(a, x, x.wide, c, h);
     }
 }
 
@@ -181,7 +310,7 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const signed char *m
 }
 
 // ---------------------------------------------------------------- norm
-constexpr int kNormChunk = 16384;      // elements of a workgroup
+constexpr int kNormChunk = 8192;       // elements of a workgroup
 struct NormTensor {
     const void *g;
     long long n;
@@ -210,21 +339,41 @@ __device__ __forceinline__ double block_sum(double s, double *lds)
 template <int DT> __device__ __forceinline__ double chunk_square(const NormTensor &t, long long begin)
 {
     constexpr unsigned kMask = DT == DDCN_F32 ? 15u : 7u;
+    constexpr int kAhead = 8;          // wide loads in flight
     const bool vec = ((unsigned long long)t.g & kMask) == 0;
     const long long end = min(t.n, begin + kNormChunk);
-    double s = 0.;
-    for (long long i = begin + threadIdx.x * 4; i < end; i += 4 * 256) {
-        float x[4];
-        load_some<DT>(t.g, i, (int)min(end - i, 4LL), vec, x);
-        for (int e = 0; e < 4; ++e) s += (double)x[e] * (double)x[e];
+    double s[4] = {0., 0., 0., 0.};
+    if (vec && begin + kNormChunk <= t.n) {
+#pragma unroll
+        for (int k = 0; k < kNormChunk / 1024; k += kAhead) {
+            float x[kAhead][4];
+#pragma unroll
+            for (int l = 0; l < kAhead; ++l) load_four<DT>(t.g, begin + (k + l) * 1024 + threadIdx.x * 4, x[l]);
+#pragma unroll
+            for (int l = 0; l < kAhead; ++l)
+                for (int e = 0; e < 4; ++e) s[e] = fma((double)x[l][e], (double)x[l][e], s[e]);
+        }
+    } else {
+        for (long long i = begin + threadIdx.x * 4; i < end; i += 1024) {
+            float x[4];
+            load_some<DT>(t.g, i, (int)min(end - i, 4LL), vec, x);
+            for (int e = 0; e < 4; ++e) s[e] = fma((double)x[e], (double)x[e], s[e]);
+        }
     }
-    return s;
+    return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 __global__ __launch_bounds__(256) void norm_partial_kernel(const NormArgs a)
 {
     __shared__ double lds[4];
-    const NormTensor &t = a.t[find_tensor(a, blockIdx.x)];
+    // the last tensor whose first workgroup is not behind this one, 64 compared at once
+    const int lane = threadIdx.x & 63;
+    int j = -1;
+    for (int i = 0; i < 3; ++i) {
+        const unsigned c0 = lane + 64 * i < a.count ? a.t[min(lane + 64 * i, kMaxNorm - 1)].chunk0 : 0xFFFFFFFFu;
+        j += __popcll(__ballot(c0 <= blockIdx.x));
+    }
+    const NormTensor &t = a.t[j];
     const long long begin = (long long)(blockIdx.x - t.chunk0) * kNormChunk;
     double s = t.dtype == DDCN_F32 ? chunk_square<DDCN_F32>(t, begin)
                : t.dtype == DDCN_BF16 ? chunk_square<DDCN_BF16>(t, begin) : chunk_square<DDCN_F16>(t, begin);
@@ -243,10 +392,17 @@ __global__ __launch_bounds__(1024) void norm_final_kernel(const double *partial,
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-template <int DT> void launch_adamw(int bits, unsigned grid, const AdamwArgs &a, hipStream_t s)
+// Blocks per wave.  fp32 moments: one (the large launch of ResNet-50's 41 M parameters takes 185 us, 190 with two or four).
+// 8 bits: two, whose loads then hide behind the other's arithmetic (107 us; 123 with one, 110 with four) -- but one where
+// two would leave CUs without work.
+constexpr unsigned kSpreadBlocks = 8192;
+template <int DT, int BITS> void launch_adamw(const AdamwArgs &a, hipStream_t s)
 {
-    if (bits == 32) adamw_kernel<DT, 32><<<grid, 64 * kWaves, 0, s>>>(a);
-    else adamw_kernel<DT, 8><<<grid, 64 * kWaves, 0, s>>>(a);
+    constexpr int kMany = BITS == 32 ? 1 : 2;
+    if (kMany == 1 || a.blocks <= kSpreadBlocks)
+        adamw_kernel<DT, BITS, 1><<<(unsigned)ceil_div(a.blocks, kWaves), 64 * kWaves, 0, s>>>(a);
+    else
+        adamw_kernel<DT, BITS, kMany><<<(unsigned)ceil_div(a.blocks, kMany * kWaves), 64 * kWaves, 0, s>>>(a);
 }
 
 }  // namespace
@@ -306,45 +462,52 @@ int ddcn_adamw_step(int count, const unsigned long long *params, const unsigned 
     a.max_norm = grad_norm ? (float)h->max_norm : 0.f;
     a.seed = h->seed;
     a.count = 0;
-    long long chunks = 0, block = 0;
+    a.blocks = 0;
+    a.first = 0;
+    a.step_size = a.rsqrt_bc2 = 0.f;
+    long long block = 0;
     int known = 0;
-    float step_size = 0.f, rsqrt_bc2 = 0.f;
-    for (int i = 0; i <= count; ++i) {
-        const bool end = i == count;
-        const long long blocks = end ? 0 : ceil_div(numels[i], kBlock), mine = ceil_div(blocks, kChunkBlocks);
-        if (a.count && (end || a.count == kMaxTensors || chunks + mine >= (1LL << 31))) {
-            const unsigned grid = (unsigned)chunks;
+    bool any = false;          // a gradient among the launch's tensors
+    auto launch = [&]() -> int {
+        const bool due = any;
+        any = false;
+        if (due) {
             hipStream_t s = (hipStream_t)stream;
-            if (h->dtype == DDCN_F32) launch_adamw<DDCN_F32>(h->bits, grid, a, s);
-            else if (h->dtype == DDCN_BF16) launch_adamw<DDCN_BF16>(h->bits, grid, a, s);
-            else launch_adamw<DDCN_F16>(h->bits, grid, a, s);
-            const int rc = check_launch("adamw");
+            if (h->dtype == DDCN_F32) h->bits == 32 ? launch_adamw<DDCN_F32, 32>(a, s) : launch_adamw<DDCN_F32, 8>(a, s);
+            else if (h->dtype == DDCN_BF16) h->bits == 32 ? launch_adamw<DDCN_BF16, 32>(a, s) : launch_adamw<DDCN_BF16, 8>(a, s);
+            else h->bits == 32 ? launch_adamw<DDCN_F16, 32>(a, s) : launch_adamw<DDCN_F16, 8>(a, s);
+        }
+        a.count = 0;
+        a.blocks = 0;
+        a.first = block;
+        return due ? check_launch("adamw") : DDCN_OK;
+    };
+    for (int i = 0; i < count; ++i) {
+        const int step = steps ? steps[i] : h->step;
+        if (step != known) {       // one step number to a launch
+            const int rc = launch();
             if (rc != DDCN_OK) return rc;
-            a.count = 0;
-            chunks = 0;
+            a.step_size = (float)(h->lr / (1.0 - pow(h->beta1, step)));
+            a.rsqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow(h->beta2, step)));
+            known = step;
         }
-        if (end) break;
-        if (blocks && grads[i]) {
-            if (mine >= (1LL << 31)) return fail(DDCN_ERR_UNSUPPORTED, "tensor %d has more than 2^43 elements", i);
-            const int step = steps ? steps[i] : h->step;
-            if (step != known) {
-                step_size = (float)(h->lr / (1.0 - pow(h->beta1, step)));
-                rsqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow(h->beta2, step)));
-                known = step;
+        // a tensor of 2^31 elements and more goes in pieces
+        for (long long done = 0; done < numels[i]; done += 1LL << 31) {
+            const long long n = numels[i] - done < (1LL << 31) ? numels[i] - done : 1LL << 31, blocks = ceil_div(n, kBlock);
+            if (a.count == kMaxTensors || a.blocks + blocks > (1LL << 31)) {
+                const int rc = launch();
+                if (rc != DDCN_OK) return rc;
             }
-            AdamwTensor &t = a.t[a.count++];
-            t.p = (void *)params[i];
-            t.g = (const void *)grads[i];
-            t.n = numels[i];
-            t.block0 = (unsigned)block;
-            t.chunk0 = (unsigned)chunks;
-            t.step_size = step_size;
-            t.rsqrt_bc2 = rsqrt_bc2;
-            chunks += mine;
+            a.p[a.count] = (void *)(params[i] + done * size);
+            a.g[a.count] = grads[i] ? (const void *)(grads[i] + done * size) : nullptr;
+            a.block0[a.count] = a.blocks;
+            a.n[a.count++] = (unsigned)n;
+            a.blocks += (unsigned)blocks;
+            block += blocks;
+            any = any || grads[i];
         }
-        block += blocks;
     }
-    return DDCN_OK;
+    return launch();
 }
 
 int ddcn_adamw_moments(const void *exp_avg, const void *exp_avg_sq, const float *exp_avg_scale,

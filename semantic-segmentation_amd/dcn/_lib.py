@@ -170,5 +170,27 @@ def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+class _Nothing:
+    """`on_device` where nothing has to change."""
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NOTHING = _Nothing()
+
+
+def on_device(index):
+    """torch.cuda.device(index), without its cost where `index` is the current device already."""
+    return _NOTHING if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def stream_of(index):
+    """The current stream of GPU `index` as the C ABI takes it (no Stream object is made)."""
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
+
+
 def current_stream(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)

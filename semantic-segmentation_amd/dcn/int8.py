@@ -53,10 +53,11 @@ def _weight_rows(weight_q):
 def _product(x, y, weight_q, weight_scale, bias, geom):
     L = _lib.lib()
     nbytes = L.ddcn_int8_workspace_bytes(geom)
-    with torch.cuda.device(x.device):
+    dev = x.get_device()
+    with _lib.on_device(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         _lib.check(L.ddcn_int8_product(_lib.ptr(x), _lib.ptr(weight_q), _lib.ptr(weight_scale), _lib.ptr(bias),
-                                       _lib.ptr(y), _lib.ptr(ws), nbytes, geom, _lib.current_stream(x.device)))
+                                       _lib.ptr(y), _lib.ptr(ws), nbytes, geom, _lib.stream_of(dev)))
     return y
 
 
@@ -79,9 +80,10 @@ def quantize_int8(x):
     q = torch.empty((rows, k), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     g = _lib.Int8Geom(1, rows, 1, k, 1, 0, _lib.ELEMENT_TYPES[x.dtype], 0, 0, 0, x.stride(0), 0, 1, k)
-    with torch.cuda.device(x.device):
+    dev = x.get_device()
+    with _lib.on_device(dev):
         _lib.check(_lib.lib().ddcn_int8_quantize(_lib.ptr(x), _lib.ptr(q), k, _lib.ptr(scale), g,
-                                                 _lib.current_stream(x.device)))
+                                                 _lib.stream_of(dev)))
     return q, scale
 
 
