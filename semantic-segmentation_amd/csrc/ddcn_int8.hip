@@ -1,9 +1,15 @@
 // Linear layers and 1x1 convolutions in 8-bit integers, a scale per token and per output channel (gfx950).  The formulas
 // stand in include/ddcn_hip.h.
 //
-//   quantize_rows / quantize_map   x (any strides) -> q int8 [token][ldq], zero from k to ldq, and the tokens' scales
-//   product                        q x weight^T on v_mfma_i32_16x16x64_i8, exact int32 sums, scales + bias + ReLU in the
-//                                  epilogue
+//   prepare_*    x (any strides) -> codes and the tokens' scales; workgroups behind those of the tokens repack the weights
+//   gemm8        codes x weights on v_mfma_i32_16x16x64_i8, operands global -> LDS by DMA through a ring of K steps; exact
+//                int32 sums, scales + bias + ReLU in the epilogue, or int32 partial sums where K is split
+//   gemv8        up to 16 tokens: a wave per channel streams its weights once, v_dot4_i32_i8
+//   finish       sums of the partial sums, epilogue
+//
+// Codes and repacked weights are stored as [k / 16][token or channel][16]: sixteen consecutive k of one row are one operand
+// fragment of the MFMA, rows follow each other.  A DMA request of 64 lanes is then 1 KB in a row, the LDS image needs no
+// swizzle, and both preparing kernels write whole lines.  k is padded with zeros to whole K steps of 64.
 #include "ddcn_elem.h"
 
 namespace ddcn {
@@ -11,140 +17,453 @@ namespace {
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 
-constexpr int kPadK = 128;             // rows of q are padded to this many bytes
 constexpr int kMaxK = 131072;          // k * 127 * 128 stays below 2^31
+constexpr long long kPassTokens = 1LL << 24;   // tokens of one pass: offsets within four rows of chunks fit 31 bits
 
 struct Int8Args {
     const void *x;
-    signed char *q;
-    float *scale;
+    u32x4 *q;                          // codes [chunks][ldq]
+    float *scale;                      // [tokens of the pass]
+    signed char *q_rows;               // ddcn_int8_quantize: codes [token][ldq] instead
     const signed char *w;
+    u32x4 *wp;                         // repacked weights [chunks][channels]
     const float *w_scale, *bias;
     void *y;
-    long long tokens, plane;           // plane = rows * cols
+    int *part;                         // partial sums [split][rows][cols]
+    long long t0;                      // first token of the pass
     long long si, sh, sw, sk, ldq, ldw;
-    int k, channels, cols, relu;
+    int tokens;                        // of the pass
+    int plane, cols;                   // of an image
+    int k, chunks, channels, relu;     // chunks: of 16 k, whole K steps
+    int prep_blocks;                   // workgroups of the tokens; the rest repack weights
+    int steps_per;                     // K steps of a split
 };
 
-// first element of token t in x
-__device__ __forceinline__ long long token_base(const Int8Args &a, long long t)
+// first element of token t (of the pass) in x
+__device__ __forceinline__ long long token_base(const Int8Args &a, int t)
 {
-    const long long img = t / a.plane, p = t - img * a.plane;
-    const long long h = p / a.cols;
-    return img * a.si + h * a.sh + (p - h * a.cols) * a.sw;
+    const unsigned u = (unsigned)(a.t0 + t), img = u / (unsigned)a.plane, p = u - img * (unsigned)a.plane;
+    const unsigned h = p / (unsigned)a.cols;
+    return img * a.si + h * a.sh + (p - h * (unsigned)a.cols) * a.sw;
 }
 
-// Scale and factor from the largest |x| of a token, given as its bits (ordered as the numbers are, NaN on top)
+// Scale and factor from the largest |x| of a token, given as its bits (ordered as the numbers are, NaN on top).  Factor 0
+// marks a token with a NaN or an infinity: its codes are 0 and its scale is NaN.
 __device__ __forceinline__ void token_scale(unsigned top, float &scale, float &factor)
 {
     constexpr unsigned kLeast = 0x0F800000u, kInf = 0x7F800000u;      // 2^-96
-    if (top >= kInf) {
-        scale = __uint_as_float(0x7FC00000u);
-        factor = 0.f;
-        return;
-    }
     const float m = __uint_as_float(max(top, kLeast));
-    scale = m / 127.f;
-    factor = 127.f / m;
+    scale = top >= kInf ? __uint_as_float(0x7FC00000u) : m / 127.f;
+    factor = top >= kInf ? 0.f : 127.f / m;
 }
-// one code; factor 0 marks a token with a NaN or an infinity: its codes are 0 and its scale is NaN
+__device__ __forceinline__ unsigned bits_of(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// Adding 1.5 * 2^23 rounds to the nearest even whole number and leaves it in the low bits: the product is rounded to fp32
+// first, as the code is defined.  (NaN and infinity times 0 leave other bits there: masked by `fine`.)
 __device__ __forceinline__ unsigned code(float x, float factor)
 {
-    return factor > 0.f ? (unsigned)(int)rintf(x * factor) & 255u : 0u;
+#pragma clang fp contract(off)
+    const float v = x * factor;
+    return __float_as_uint(v + 12582912.f) & 255u;
+}
+__device__ __forceinline__ u32x4 pack16(const float (&x)[16], float factor)
+{
+    u32x4 r;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+        r[d] = code(x[4 * d], factor) | code(x[4 * d + 1], factor) << 8 | code(x[4 * d + 2], factor) << 16 | code(x[4 * d + 3], factor) << 24;
+    const unsigned fine = factor > 0.f ? ~0u : 0u;
+    return u32x4{r[0] & fine, r[1] & fine, r[2] & fine, r[3] & fine};
 }
 
-// sk == 1: a wave per token
-template <int DT> __global__ __launch_bounds__(256) void quantize_rows_kernel(const Int8Args a)
+// ---------------------------------------------------------------- weights
+// 16 weight bytes from k on, zero behind the row's kk bytes
+__device__ __forceinline__ u32x4 weight_chunk(const signed char *row, int k, int kk, bool wide)
 {
-    const int lane = threadIdx.x & 63;
-    const long long t = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= a.tokens) return;
-    const long long base = token_base(a, t);
-    unsigned top = 0;
-    for (int k = lane; k < a.k; k += 64) top = max(top, __float_as_uint(fabsf(load_one<DT>(a.x, base + k))));
-    for (int d = 32; d; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
-    float scale, factor;
-    token_scale(top, scale, factor);
-    signed char *q = a.q + t * a.ldq;
-    for (long long k = lane; k < a.ldq; k += 64) q[k] = k < a.k ? (signed char)code(load_one<DT>(a.x, base + k), factor) : 0;
-    if (lane == 0) a.scale[t] = scale;
+    if (wide && k + 16 <= kk) return *(const u32x4 *)(row + k);
+    unsigned u[4] = {0u, 0u, 0u, 0u};
+    for (int e = 0; e < 16; ++e)
+        if (k + e < kk) u[e >> 2] |= (unsigned)(unsigned char)row[k + e] << (8 * (e & 3));
+    return u32x4{u[0], u[1], u[2], u[3]};
+}
+__device__ __forceinline__ bool wide_rows(const Int8Args &a) { return (((unsigned long long)a.w | (unsigned long long)a.ldw) & 15) == 0; }
+
+// A wave moves 8 rows x 8 chunks: 128-byte lines on both sides
+__device__ __forceinline__ void repack_weights(const Int8Args &a, int block, int blocks)
+{
+    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int across = (a.chunks + 7) / 8, items = (a.channels + 7) / 8 * across;
+    const bool wide = wide_rows(a);
+    for (int i = block * waves + (threadIdx.x >> 6); i < items; i += blocks * waves) {
+        const int n = i / across * 8 + (lane & 7), c = i % across * 8 + (lane >> 3);
+        if (n < a.channels && c < a.chunks)
+            a.wp[(long long)c * a.channels + n] = weight_chunk(a.w + n * a.ldw, c * 16, a.k, wide);
+    }
 }
 
-// any strides, lanes along the tokens: 64 tokens per workgroup, the channels dealt to its four waves
-template <int DT> __global__ __launch_bounds__(256) void quantize_map_kernel(const Int8Args a)
+// ---------------------------------------------------------------- tokens
+__device__ __forceinline__ void store_chunk(const Int8Args &a, int t, int c, u32x4 v)
 {
-    __shared__ unsigned tops[4][64];
+    if (!a.q_rows) {
+        a.q[(long long)c * a.ldq + t] = v;
+    } else {                                               // rows of bytes: only what exists
+        signed char *row = a.q_rows + (a.t0 + t) * a.ldq;
+        for (int e = 0; e < 16; ++e)
+            if (c * 16 + e < a.ldq) row[c * 16 + e] = (signed char)(v[e >> 2] >> (8 * (e & 3)));
+    }
+}
+
+template <int DT> __device__ __forceinline__ void load_16(const Int8Args &a, long long base, int k, bool vec, float (&x)[16])
+{
+    if (vec && k + 16 <= a.k) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            float f[4];
+            if (DT == DDCN_F32) load_four<DT>(a.x, base + k + 4 * d, f);
+            else if (d & 1) continue;
+            else {
+                const u32x4 u = *(const u32x4 *)((const bf16_t *)a.x + base + k + 4 * d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[4 * d + 2 * e] = DT == DDCN_BF16 ? BF16::lo(u[e]) : F16::lo(u[e]);
+                    x[4 * d + 2 * e + 1] = DT == DDCN_BF16 ? BF16::hi(u[e]) : F16::hi(u[e]);
+                }
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * d + e] = f[e];
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = k + e < a.k ? load_one<DT>(a.x, base + (k + e) * a.sk) : 0.f;
+}
+
+// sk == 1: W waves per token, 16 consecutive values per lane and turn, up to I turns held in registers (more are read again)
+template <int DT, int W, int I> __global__ __launch_bounds__(256) void prepare_rows_kernel(const Int8Args a)
+{
+    if ((int)blockIdx.x >= a.prep_blocks) return repack_weights(a, blockIdx.x - a.prep_blocks, gridDim.x - a.prep_blocks);
+    __shared__ unsigned tops[4];
+    constexpr int kTurn = 64 * W;                          // chunks of a turn
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long t = (long long)blockIdx.x * 64 + lane;
+    const int t = blockIdx.x * (4 / W) + wave / W, first = (wave % W) * 64 + lane;
     const bool live = t < a.tokens;
     const long long base = live ? token_base(a, t) : 0;
+    constexpr int kAlign = DT == DDCN_F32 ? 4 : 8;
+    const bool vec = (base & (kAlign - 1)) == 0 && ((unsigned long long)a.x & 15) == 0;
+    float x[I][16];
     unsigned top = 0;
-    if (live)
-        for (int k = wave; k < a.k; k += 4) top = max(top, __float_as_uint(fabsf(load_one<DT>(a.x, base + k * a.sk))));
-    tops[wave][lane] = top;
-    __syncthreads();
-    top = max(max(tops[0][lane], tops[1][lane]), max(tops[2][lane], tops[3][lane]));
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+            if (first + i * kTurn < a.chunks) load_16<DT>(a, base, (first + i * kTurn) * 16, vec, x[i]);
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+            if (first + i * kTurn < a.chunks)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = max(top, bits_of(x[i][e]));
+        for (int c = first + I * kTurn; c < a.chunks; c += kTurn) {
+            float z[16];
+            load_16<DT>(a, base, c * 16, vec, z);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = max(top, bits_of(z[e]));
+        }
+    }
+    for (int d = 32; d; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
+    if (W > 1) {
+        if (lane == 0) tops[wave] = top;
+        __syncthreads();
+        top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    }
     if (!live) return;
     float scale, factor;
     token_scale(top, scale, factor);
-    signed char *q = a.q + t * a.ldq;
-    for (long long k = wave; k < a.ldq; k += 4)
-        q[k] = k < a.k ? (signed char)code(load_one<DT>(a.x, base + k * a.sk), factor) : 0;
-    if (wave == 0) a.scale[t] = scale;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+        if (first + i * kTurn < a.chunks) store_chunk(a, t, first + i * kTurn, pack16(x[i], factor));
+    for (int c = first + I * kTurn; c < a.chunks; c += kTurn) {
+        float z[16];
+        load_16<DT>(a, base, c * 16, vec, z);
+        store_chunk(a, t, c, pack16(z, factor));
+    }
+    if (first == 0) a.scale[a.q_rows ? a.t0 + t : t] = scale;
 }
 
-// 16 weight bytes from k on, zero behind the row's k bytes
-__device__ __forceinline__ i32x4 weight_chunk(const signed char *row, int k, int kk, bool wide)
+// Any strides, lanes along the tokens: 32 tokens per workgroup, half a wave per chunk of 16 channels, I chunks per half
+// wave held in registers (more are read again)
+template <int DT, int NT, int I> __global__ __launch_bounds__(NT) void prepare_map_kernel(const Int8Args a)
 {
-    if (wide && k + 16 <= kk) return *(const i32x4 *)(row + k);
-    union {
-        signed char b[16];
-        i32x4 v;
-    } u;
-    for (int e = 0; e < 16; ++e) u.b[e] = k + e < kk ? row[k + e] : 0;
-    return u.v;
+    if ((int)blockIdx.x >= a.prep_blocks) return repack_weights(a, blockIdx.x - a.prep_blocks, gridDim.x - a.prep_blocks);
+    constexpr int kHalves = NT / 32;
+    __shared__ unsigned tops[NT / 64][32];
+    const int tl = threadIdx.x & 31, half = threadIdx.x >> 5;
+    const int t = blockIdx.x * 32 + tl;
+    const bool live = t < a.tokens;
+    const long long base = live ? token_base(a, t) : 0;
+    float x[I][16];
+    unsigned top = 0;
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+            if (half + i * kHalves < a.chunks) load_16<DT>(a, base, (half + i * kHalves) * 16, false, x[i]);
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+            if (half + i * kHalves < a.chunks)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = max(top, bits_of(x[i][e]));
+        for (int c = half + I * kHalves; c < a.chunks; c += kHalves) {
+            float z[16];
+            load_16<DT>(a, base, c * 16, false, z);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = max(top, bits_of(z[e]));
+        }
+    }
+    top = max(top, (unsigned)__shfl_xor((int)top, 32));
+    if ((threadIdx.x & 32) == 0) tops[threadIdx.x >> 6][tl] = top;
+    __syncthreads();
+    for (int w = 0; w < NT / 64; ++w) top = max(top, tops[w][tl]);
+    if (!live) return;
+    float scale, factor;
+    token_scale(top, scale, factor);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+        if (half + i * kHalves < a.chunks) store_chunk(a, t, half + i * kHalves, pack16(x[i], factor));
+    for (int c = half + I * kHalves; c < a.chunks; c += kHalves) {
+        float z[16];
+        load_16<DT>(a, base, c * 16, false, z);
+        store_chunk(a, t, c, pack16(z, factor));
+    }
+    if (half == 0) a.scale[a.q_rows ? a.t0 + t : t] = scale;
 }
 
-// 64 x 64 per workgroup, 32 x 32 per wave.  The operand whose index runs along the lanes of the result is the one that is
-// contiguous in y: tokens for nchw, channels otherwise.
-template <int DT, bool NCHW> __global__ __launch_bounds__(256) void product_kernel(const Int8Args a)
+// ---------------------------------------------------------------- epilogue
+__device__ __forceinline__ float finished(const Int8Args &a, int sum, float st, float sn, float bias)
 {
 #pragma clang fp contract(off)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long t0 = (long long)blockIdx.x * 64 + (wave & 1) * 32;
-    const int n0 = blockIdx.y * 64 + (wave >> 1) * 32;
-    const int r16 = lane & 15, kc = (lane >> 4) * 16;
-    const bool wide = (((unsigned long long)a.w | (unsigned long long)a.ldw) & 15) == 0;
-    i32x4 acc[2][2] = {};
-    const i32x4 zero = {0, 0, 0, 0};
-    for (int k0 = 0; k0 < a.k; k0 += 64) {
-        i32x4 ft[2], fw[2];
-        for (int i = 0; i < 2; ++i) {
-            const long long t = t0 + i * 16 + r16;
-            const int n = n0 + i * 16 + r16;
-            ft[i] = t < a.tokens ? *(const i32x4 *)(a.q + t * a.ldq + k0 + kc) : zero;
-            fw[i] = n < a.channels ? weight_chunk(a.w + n * a.ldw, k0 + kc, a.k, wide) : zero;
-        }
-        for (int i = 0; i < 2; ++i)
-            for (int j = 0; j < 2; ++j)
-                acc[i][j] = NCHW ? __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], ft[j], acc[i][j], 0, 0, 0)
-                                 : __builtin_amdgcn_mfma_i32_16x16x64_i8(ft[i], fw[j], acc[i][j], 0, 0, 0);
+    float v = (float)sum * (st * sn);
+    if (a.bias) v = v + bias;
+    return a.relu && v < 0.f ? 0.f : v;                    // a NaN stays
+}
+// where token t (of the pass), channel 0 lies in y, and the stride of the channels
+template <bool NCHW> __device__ __forceinline__ long long out_base(const Int8Args &a, int t)
+{
+    const unsigned u = (unsigned)(a.t0 + t);
+    if (!NCHW) return (long long)u * a.channels;
+    const unsigned img = u / (unsigned)a.plane;
+    return (long long)img * a.channels * a.plane + (u - img * (unsigned)a.plane);
+}
+
+// ---------------------------------------------------------------- product
+// Workgroups round-robin over the 8 XCDs by launch index: give each XCD a contiguous run of tiles (bijective)
+__device__ __forceinline__ int xcd_logical(int b, int total)
+{
+    const int q = total / 8, r = total % 8, xcd = b % 8, k = b / 8;
+    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + k;
+}
+
+// N requests of 16 bytes per lane from `from` (`bytes` readable there), to LDS STEP bytes apart
+template <int N, int STEP> __device__ __forceinline__ void dma(const u32x4 *from, unsigned bytes, char *to, const unsigned *off)
+{
+    const __amdgpu_buffer_rsrc_t r = uniform_rsrc(from, bytes);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(to + i * STEP), 16, off[i], 0, 0, 0);
+}
+
+__device__ __forceinline__ i32x4 mfma8(u32x4 a, u32x4 b, i32x4 c)
+{
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
+
+// Rows of the tile run along the registers of the result, columns along its lanes; the columns are what is contiguous in y:
+// tokens for nchw (rows: channels), channels otherwise (rows: tokens).  Tile 2*MI*32 rows x 64*NWN columns, 2 x NWN waves of
+// MI*32 x 64.  A ring of NS K steps (64 k each) in LDS, filled by DMA: request of step s + NS goes into the stage that step s
+// has left.  One barrier per step, between the two halves of its MFMAs: fragments are read one half ahead of their use.
+template <int DT, bool NCHW, bool PART, int MI, int NWN, int NS>
+__global__ __launch_bounds__(128 * NWN, NWN == 4 ? 1 : 2) void gemm8_kernel(const Int8Args a)
+{
+    constexpr int NT = 128 * NWN, NWAVES = NT / 64, BR = 2 * MI * 32, BC = 64 * NWN;
+    constexpr int RR = BR * 4 / NT, RC = BC * 4 / NT;      // requests per thread and step
+    constexpr int STAGE = BR * 4 + BC * 4;                 // 16-byte chunks of a stage
+    extern __shared__ u32x4 ring[];
+    const int t = threadIdx.x, lane = t & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int wr = wave / NWN, wc = wave % NWN;
+    const int rows = NCHW ? a.channels : a.tokens, cols = NCHW ? a.tokens : a.channels;
+    const u32x4 *R = NCHW ? a.wp : a.q, *C = NCHW ? a.q : a.wp;
+    const long long ldr = NCHW ? a.channels : a.ldq, ldc = NCHW ? a.ldq : a.channels;
+    const int tiles_r = (rows + BR - 1) / BR, tiles_c = (cols + BC - 1) / BC;
+    const int L = xcd_logical(blockIdx.x, tiles_r * tiles_c);
+    // neighbours share the tile of tokens, the larger operand
+    const int r0 = (NCHW ? L % tiles_r : L / tiles_c) * BR, c0 = (NCHW ? L / tiles_r : L % tiles_c) * BC;
+    const int first = blockIdx.y * a.steps_per, steps = min(a.steps_per, a.chunks / 4 - first);
+
+    unsigned off_r[RR], off_c[RC];
+#pragma unroll
+    for (int i = 0; i < RR; ++i) {
+        const int q = (i * NWAVES + wave) * 64 + lane, row = q % BR;
+        off_r[i] = r0 + row < rows ? (unsigned)((q / BR) * ldr + row) * 16u : DMA_OOB;
     }
+#pragma unroll
+    for (int i = 0; i < RC; ++i) {
+        const int q = (i * NWAVES + wave) * 64 + lane, col = q % BC;
+        off_c[i] = c0 + col < cols ? (unsigned)((q / BC) * ldc + col) * 16u : DMA_OOB;
+    }
+    const u32x4 *pr = R + (long long)first * 4 * ldr + r0, *pc = C + (long long)first * 4 * ldc + c0;
+    const unsigned lim_r = (unsigned)(4 * ldr - r0) * 16u, lim_c = (unsigned)(4 * ldc - c0) * 16u;
+    auto request = [&](int s) {
+        char *base = (char *)(ring + (s % NS) * STAGE) + wave * 1024;
+        dma<RR, NWAVES * 1024>(pr + (long long)s * 4 * ldr, lim_r, base, off_r);
+        dma<RC, NWAVES * 1024>(pc + (long long)s * 4 * ldc, lim_c, base + BR * 64, off_c);
+    };
+
+    constexpr int RT = 2 * MI;                             // 16-row tiles of a wave
+    i32x4 acc[RT][4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    const int r16 = lane & 15, kc = lane >> 4;
+    auto read_r = [&](int s, int h, u32x4 (&f)[MI]) {
+        const u32x4 *st = ring + (s % NS) * STAGE + kc * BR + wr * (MI * 32) + h * (MI * 16) + r16;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) f[i] = st[i * 16];
+    };
+    auto read_c = [&](int s, u32x4 (&f)[4]) {
+        const u32x4 *st = ring + (s % NS) * STAGE + BR * 4 + kc * BC + wc * 64 + r16;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = st[j * 16];
+    };
+    auto mfmas = [&](int h, const u32x4 (&fr)[MI], const u32x4 (&fc)[4]) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[h * MI + i][j] = mfma8(fr[i], fc[j], acc[h * MI + i][j]);
+    };
+    // this wave's LDS reads are done and all but its `younger` youngest steps have landed
+    auto wait_but = [&](int younger) {
+        if (younger >= 3) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(3 * (RR + RC)));
+        else if (younger == 2) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(2 * (RR + RC)));
+        else if (younger == 1) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(RR + RC));
+        else __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+    };
+    static_assert(NS <= 4 && 3 * (RR + RC) < 64, "vmcnt is 6 bits and wait_but knows up to 3 steps in flight");
+    u32x4 f0[MI], f1[MI], fx[4], fy[4];
+    auto step = [&](int s, u32x4 (&fc)[4], u32x4 (&fn)[4]) {
+        read_r(s, 1, f1);
+        __builtin_amdgcn_sched_barrier(0);
+        mfmas(0, f0, fc);
+        __builtin_amdgcn_sched_barrier(0);
+        if (s + 1 < steps) {
+            wait_but(min(NS - 2, steps - 2 - s));
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            if (s + NS < steps) request(s + NS);
+            read_c(s + 1, fn);
+            read_r(s + 1, 0, f0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        mfmas(1, f1, fc);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+        if (s < steps) request(s);
+    wait_but(min(NS - 1, steps - 1));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read_c(0, fx);
+    read_r(0, 0, f0);
+    for (int s = 0; s < steps; s += 2) {
+        step(s, fx, fy);
+        if (s + 1 < steps) step(s + 1, fy, fx);
+    }
+
     // lane l holds rows 4 * (l / 16) + e, column l % 16 of each 16 x 16 tile
-    for (int i = 0; i < 2; ++i)
-        for (int j = 0; j < 2; ++j)
+    const int row0 = r0 + wr * (MI * 32) + kc * 4, col0 = c0 + wc * 64 + r16;
+    if (PART) {
+        int *part = a.part + (long long)blockIdx.y * rows * cols;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int along = j * 16 + r16, across = i * 16 + (lane >> 4) * 4 + e;
-                const long long t = t0 + (NCHW ? along : across);
-                const int n = n0 + (NCHW ? across : along);
-                if (t >= a.tokens || n >= a.channels) continue;
-                float v = (float)acc[i][j][e] * (a.scale[t] * a.w_scale[n]);
-                if (a.bias) v = v + a.bias[n];
-                if (a.relu && v < 0.f) v = 0.f;
-                const long long img = t / a.plane;
-                const long long at = NCHW ? (img * a.channels + n) * a.plane + (t - img * a.plane) : t * a.channels + n;
-                store_one<DT>(a.y, at, v);
+                const int row = row0 + i * 16 + e;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (row < rows && col0 + j * 16 < cols) part[(long long)row * cols + col0 + j * 16] = acc[i][j][e];
             }
+        return;
+    }
+    float sc[4], bc[4];
+    long long at[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int col = min(col0 + j * 16, cols - 1);
+        sc[j] = NCHW ? a.scale[col] : a.w_scale[col];
+        bc[j] = !NCHW && a.bias ? a.bias[col] : 0.f;
+        at[j] = NCHW ? out_base<true>(a, col) : col;
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = row0 + i * 16 + e;
+            if (row >= rows) continue;
+            const float sr = NCHW ? a.w_scale[row] : a.scale[row], br = NCHW && a.bias ? a.bias[row] : 0.f;
+            const long long ro = NCHW ? (long long)row * a.plane : out_base<false>(a, row);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col0 + j * 16 < cols)
+                    store_one<DT>(a.y, ro + at[j], finished(a, acc[i][j][e], NCHW ? sc[j] : sr, NCHW ? sr : sc[j], NCHW ? br : bc[j]));
+        }
+}
+
+// sums [split][rows][cols] -> y
+template <int DT, bool NCHW> __global__ __launch_bounds__(256) void finish_kernel(const Int8Args a, int splits)
+{
+    const int rows = NCHW ? a.channels : a.tokens, cols = NCHW ? a.tokens : a.channels;
+    const long long total = (long long)rows * cols, i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    int sum = 0;
+    for (int s = 0; s < splits; ++s) sum += a.part[s * total + i];
+    const int row = (int)(i / cols), col = (int)(i - (long long)row * cols);
+    const int tok = NCHW ? col : row, n = NCHW ? row : col;
+    store_one<DT>(a.y, out_base<NCHW>(a, tok) + (NCHW ? (long long)n * a.plane : n),
+                  finished(a, sum, a.scale[tok], a.w_scale[n], a.bias ? a.bias[n] : 0.f));
+}
+
+// ---------------------------------------------------------------- few tokens
+// A wave per channel, TOK tokens: the weights are read once, straight from the caller's rows, 16 bytes per lane and turn;
+// the codes of a chunk lie next to each other and come from the caches.
+template <int DT, bool NCHW, int TOK> __global__ __launch_bounds__(256) void gemv8_kernel(const Int8Args a)
+{
+    const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n >= a.channels) return;
+    const bool wide = wide_rows(a);
+    const signed char *row = a.w + n * a.ldw;
+    int acc[TOK] = {};
+#pragma unroll 4
+    for (int c = lane; c < a.chunks; c += 64) {
+        const u32x4 w = weight_chunk(row, c * 16, a.k, wide);
+#pragma unroll
+        for (int t = 0; t < TOK; ++t) {
+            const u32x4 q = a.q[(long long)c * a.ldq + min(t, a.tokens - 1)];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[t] = __builtin_amdgcn_sdot4((int)w[d], (int)q[d], acc[t], false);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TOK; ++t)
+        for (int d = 32; d; d >>= 1) acc[t] += __shfl_xor(acc[t], d);
+    // lane t writes token t
+    int sum = acc[0];
+#pragma unroll
+    for (int t = 1; t < TOK; ++t) sum = lane == t ? acc[t] : sum;
+    if (lane >= a.tokens) return;
+    store_one<DT>(a.y, out_base<NCHW>(a, lane) + (NCHW ? (long long)n * a.plane : n),
+                  finished(a, sum, a.scale[lane], a.w_scale[n], a.bias ? a.bias[n] : 0.f));
 }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -167,40 +486,116 @@ int check(const ddcn_int8_geom *g, bool product)
 }
 
 long long tokens_of(const ddcn_int8_geom *g) { return (long long)g->images * g->rows * g->cols; }
-size_t q_bytes(const ddcn_int8_geom *g) { return round_up((size_t)tokens_of(g) * round_up(g->k, kPadK), 256); }
 
-int run_quantize(const Int8Args &a, int dtype, hipStream_t s)
+// How a pass of `tokens` tokens is computed
+struct Plan {
+    bool gemv;
+    int tile;              // 0: 256 x 256, 1: 128 x 128, 2: 64 x 64
+    int splits, steps_per;
+    size_t q_bytes, scale_bytes, w_bytes, part_bytes;
+    size_t bytes() const { return q_bytes + scale_bytes + w_bytes + part_bytes; }
+};
+
+constexpr int kCUs = 256;
+constexpr int kGemvTokens = 16;
+
+Plan plan_of(const ddcn_int8_geom *g, long long tokens)
 {
-    if (a.sk == 1) {
-        const unsigned grid = (unsigned)ceil_div(a.tokens, 4);
-        if (dtype == DDCN_F32) quantize_rows_kernel<DDCN_F32><<<grid, 256, 0, s>>>(a);
-        else if (dtype == DDCN_BF16) quantize_rows_kernel<DDCN_BF16><<<grid, 256, 0, s>>>(a);
-        else quantize_rows_kernel<DDCN_F16><<<grid, 256, 0, s>>>(a);
-    } else {
-        const unsigned grid = (unsigned)ceil_div(a.tokens, 64);
-        if (dtype == DDCN_F32) quantize_map_kernel<DDCN_F32><<<grid, 256, 0, s>>>(a);
-        else if (dtype == DDCN_BF16) quantize_map_kernel<DDCN_BF16><<<grid, 256, 0, s>>>(a);
-        else quantize_map_kernel<DDCN_F16><<<grid, 256, 0, s>>>(a);
+    Plan p = {};
+    const long long chunks = ceil_div(g->k, 64) * 4, steps = chunks / 4;
+    p.q_bytes = round_up((size_t)(chunks * 16 * tokens), 256);
+    p.scale_bytes = round_up((size_t)tokens * sizeof(float), 256);
+    p.gemv = tokens <= kGemvTokens;
+    if (p.gemv) return p;
+    p.w_bytes = round_up((size_t)(chunks * 16 * g->channels), 256);
+    const long long sizes[3] = {256, 128, 64};
+    long long tiles = 0;
+    for (p.tile = 0; p.tile < 3; ++p.tile) {
+        tiles = ceil_div(tokens, sizes[p.tile]) * ceil_div(g->channels, sizes[p.tile]);
+        if (tiles >= kCUs * 3 / 4 || p.tile == 2) break;
     }
-    return check_launch("int8 quantize");
+    // K is split where the tiles leave CUs without work, into pieces of 8 steps at least
+    long long splits = tiles >= kCUs ? 1 : ceil_div(2 * kCUs, tiles);
+    if (splits > steps / 8) splits = steps / 8 > 1 ? steps / 8 : 1;
+    p.steps_per = (int)ceil_div(steps, splits);
+    p.splits = (int)ceil_div(steps, p.steps_per);
+    if (p.splits > 1) p.part_bytes = round_up((size_t)p.splits * tokens * g->channels * sizeof(int), 256);
+    return p;
 }
 
-template <bool NCHW> void run_product(const Int8Args &a, int dtype, hipStream_t s)
+template <int DT> void launch_prepare(Int8Args &a, bool repack, hipStream_t s)
 {
-    const dim3 grid((unsigned)ceil_div(a.tokens, 64), (unsigned)ceil_div(a.channels, 64));
-    if (dtype == DDCN_F32) product_kernel<DDCN_F32, NCHW><<<grid, 256, 0, s>>>(a);
-    else if (dtype == DDCN_BF16) product_kernel<DDCN_BF16, NCHW><<<grid, 256, 0, s>>>(a);
-    else product_kernel<DDCN_F16, NCHW><<<grid, 256, 0, s>>>(a);
+    // repacking: a wave moves 64 chunks; enough workgroups to take no longer than the tokens do
+    const int extra = repack ? (int)(ceil_div((long long)a.channels * a.chunks, 64 * 16) < 4096 ? ceil_div((long long)a.channels * a.chunks, 64 * 16) : 4096) : 0;
+    if (a.sk == 1) {
+        const bool many = a.chunks > 128;                  // more than 2048 values: four waves per token
+        a.prep_blocks = (int)ceil_div(a.tokens, many ? 1 : 4);
+        const unsigned grid = (unsigned)(a.prep_blocks + extra);
+        if (many) prepare_rows_kernel<DT, 4, 4><<<grid, 256, 0, s>>>(a);
+        else if (a.chunks > 64) prepare_rows_kernel<DT, 1, 2><<<grid, 256, 0, s>>>(a);
+        else prepare_rows_kernel<DT, 1, 1><<<grid, 256, 0, s>>>(a);
+    } else {
+        a.prep_blocks = (int)ceil_div(a.tokens, 32);
+        const unsigned grid = (unsigned)(a.prep_blocks + extra);
+        if (a.chunks <= 8) prepare_map_kernel<DT, 256, 1><<<grid, 256, 0, s>>>(a);
+        else if (a.chunks <= 32) prepare_map_kernel<DT, 1024, 1><<<grid, 1024, 0, s>>>(a);
+        else if (a.chunks <= 64) prepare_map_kernel<DT, 1024, 2><<<grid, 1024, 0, s>>>(a);
+        else prepare_map_kernel<DT, 1024, 4><<<grid, 1024, 0, s>>>(a);
+    }
+}
+int run_prepare(Int8Args &a, int dtype, bool repack, hipStream_t s)
+{
+    if (dtype == DDCN_F32) launch_prepare<DDCN_F32>(a, repack, s);
+    else if (dtype == DDCN_BF16) launch_prepare<DDCN_BF16>(a, repack, s);
+    else launch_prepare<DDCN_F16>(a, repack, s);
+    return check_launch("int8 prepare");
+}
+
+template <int DT, bool NCHW, bool PART, int MI, int NWN, int NS> int launch_tiles(const Int8Args &a, int splits, hipStream_t s)
+{
+    constexpr int BR = 2 * MI * 32, BC = 64 * NWN, kLds = NS * (BR + BC) * 64;
+    static std::atomic<uint64_t> done{0};
+    if (!raise_lds_limit((const void *)gemm8_kernel<DT, NCHW, PART, MI, NWN, NS>, kLds, done)) return fail(DDCN_ERR_LAUNCH, "int8 product: LDS limit");
+    const long long rows = NCHW ? a.channels : a.tokens, cols = NCHW ? a.tokens : a.channels;
+    gemm8_kernel<DT, NCHW, PART, MI, NWN, NS><<<dim3((unsigned)(ceil_div(rows, BR) * ceil_div(cols, BC)), (unsigned)splits), 128 * NWN, kLds, s>>>(a);
+    return check_launch("int8 product");
+}
+template <int DT, bool NCHW, bool PART> int launch_gemm(const Int8Args &a, const Plan &p, hipStream_t s)
+{
+    if (p.tile == 0) return launch_tiles<DT, NCHW, PART, 4, 4, 4>(a, p.splits, s);
+    if (p.tile == 1) return launch_tiles<DT, NCHW, PART, 2, 2, 4>(a, p.splits, s);
+    return launch_tiles<DT, NCHW, PART, 1, 1, 4>(a, p.splits, s);
+}
+template <int DT, bool NCHW> int launch_product(const Int8Args &a, const Plan &p, hipStream_t s)
+{
+    if (p.gemv) {
+        const unsigned grid = (unsigned)ceil_div(a.channels, 4);
+        if (a.tokens == 1) gemv8_kernel<DT, NCHW, 1><<<grid, 256, 0, s>>>(a);
+        else if (a.tokens <= 4) gemv8_kernel<DT, NCHW, 4><<<grid, 256, 0, s>>>(a);
+        else gemv8_kernel<DT, NCHW, 16><<<grid, 256, 0, s>>>(a);
+        return check_launch("int8 product");
+    }
+    if (p.splits == 1) return launch_gemm<DT, NCHW, false>(a, p, s);
+    const int rc = launch_gemm<DDCN_F32, NCHW, true>(a, p, s);
+    if (rc != DDCN_OK) return rc;
+    finish_kernel<DT, NCHW><<<(unsigned)ceil_div((long long)a.tokens * a.channels, 256), 256, 0, s>>>(a, p.splits);
+    return check_launch("int8 finish");
+}
+template <bool NCHW> int run_product(const Int8Args &a, const Plan &p, int dtype, hipStream_t s)
+{
+    if (dtype == DDCN_F32) return launch_product<DDCN_F32, NCHW>(a, p, s);
+    if (dtype == DDCN_BF16) return launch_product<DDCN_BF16, NCHW>(a, p, s);
+    return launch_product<DDCN_F16, NCHW>(a, p, s);
 }
 
 Int8Args args_of(const ddcn_int8_geom *g)
 {
     Int8Args a = {};
-    a.tokens = tokens_of(g);
-    a.plane = (long long)g->rows * g->cols;
+    a.plane = g->rows * g->cols;
     a.si = g->si; a.sh = g->sh; a.sw = g->sw; a.sk = g->sk;
     a.ldw = g->ldw;
     a.k = g->k; a.channels = g->channels; a.cols = g->cols; a.relu = g->relu;
+    a.chunks = (int)ceil_div(g->k, 64) * 4;
     return a;
 }
 
@@ -213,8 +608,9 @@ extern "C" {
 
 size_t ddcn_int8_workspace_bytes(const ddcn_int8_geom *g)
 {
-    if (check(g, false) != DDCN_OK) return 0;
-    return q_bytes(g) + round_up((size_t)tokens_of(g) * sizeof(float), 256);
+    if (check(g, true) != DDCN_OK || !tokens_of(g)) return 0;
+    const long long tokens = tokens_of(g);
+    return plan_of(g, tokens < kPassTokens ? tokens : kPassTokens).bytes();
 }
 
 int ddcn_int8_product(const void *x, const void *weight, const float *weight_scale, const float *bias, void *y,
@@ -229,33 +625,51 @@ int ddcn_int8_product(const void *x, const void *weight, const float *weight_sca
     if (workspace_bytes < need) return fail(DDCN_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
     Int8Args a = args_of(g);
     a.x = x;
-    a.q = (signed char *)workspace;
-    a.scale = (float *)((char *)workspace + q_bytes(g));
-    a.ldq = (long long)round_up(g->k, kPadK);
     a.w = (const signed char *)weight;
     a.w_scale = weight_scale;
     a.bias = bias;
     a.y = y;
-    rc = run_quantize(a, g->dtype, (hipStream_t)stream);
-    if (rc != DDCN_OK) return rc;
-    if (g->nchw) run_product<true>(a, g->out_dtype, (hipStream_t)stream);
-    else run_product<false>(a, g->out_dtype, (hipStream_t)stream);
-    return check_launch("int8 product");
+    const long long total = tokens_of(g);
+    for (a.t0 = 0; a.t0 < total; a.t0 += kPassTokens) {    // (later passes fit the first one's workspace)
+        a.tokens = (int)(total - a.t0 < kPassTokens ? total - a.t0 : kPassTokens);
+        const Plan p = plan_of(g, a.tokens);
+        char *ws = (char *)workspace;
+        a.ldq = a.tokens;
+        a.q = (u32x4 *)ws;
+        a.scale = (float *)(ws += p.q_bytes);
+        a.wp = (u32x4 *)(ws += p.scale_bytes);
+        a.part = (int *)(ws += p.w_bytes);
+        a.steps_per = p.steps_per;
+        if ((size_t)(ws - (char *)workspace) + p.part_bytes > workspace_bytes) return fail(DDCN_ERR_WORKSPACE, "workspace too small for the last pass");
+        rc = run_prepare(a, g->dtype, !p.gemv, (hipStream_t)stream);
+        if (rc != DDCN_OK) return rc;
+        rc = g->nchw ? run_product<true>(a, p, g->out_dtype, (hipStream_t)stream) : run_product<false>(a, p, g->out_dtype, (hipStream_t)stream);
+        if (rc != DDCN_OK) return rc;
+    }
+    return DDCN_OK;
 }
 
 int ddcn_int8_quantize(const void *x, void *q, long long ldq, float *scale, const ddcn_int8_geom *g, void *stream)
 {
-    const int rc = check(g, false);
+    int rc = check(g, false);
     if (rc != DDCN_OK) return rc;
     if (ldq < g->k) return fail(DDCN_ERR_SHAPE, "rows of %lld bytes hold no %d values", ldq, g->k);
+    if (ldq > g->k + 64LL) return fail(DDCN_ERR_UNSUPPORTED, "rows of %lld bytes for %d values: at most 64 of padding", ldq, g->k);
     if (!tokens_of(g)) return DDCN_OK;
     if (!x || !q || !scale) return fail(DDCN_ERR_BAD_ARG, "a pointer is NULL");
     Int8Args a = args_of(g);
     a.x = x;
-    a.q = (signed char *)q;
+    a.q_rows = (signed char *)q;
     a.ldq = ldq;
     a.scale = scale;
-    return run_quantize(a, g->dtype, (hipStream_t)stream);
+    a.chunks = (int)ceil_div(ldq, 16);
+    const long long total = tokens_of(g);
+    for (a.t0 = 0; a.t0 < total; a.t0 += kPassTokens) {
+        a.tokens = (int)(total - a.t0 < kPassTokens ? total - a.t0 : kPassTokens);
+        rc = run_prepare(a, g->dtype, false, (hipStream_t)stream);
+        if (rc != DDCN_OK) return rc;
+    }
+    return DDCN_OK;
 }
 
 }  // extern "C"

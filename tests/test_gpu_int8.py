@@ -267,3 +267,19 @@ def test_layers_from_float_ones():
     xs, w = _np(x)[:, :, ::2, ::2], _np(conv.weight)[:, :, 0, 0] * _np(norm.weight * torch.rsqrt(norm.running_var + norm.eps))[:, None]
     bound = 24 / 254 * 2.1 * np.abs(xs).max(1)[:, None] * np.abs(w).max(1)[None, :, None, None]
     assert (np.abs(y - full) <= bound).all()
+
+
+def test_more_tokens_than_one_pass():
+    """2^24 tokens and some: the second pass writes behind the first one's."""
+    t, k, n = (1 << 24) + 37, 8, 3
+    x = torch.randint(-3, 4, (t, k), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(torch.float16)
+    wq, ws, b = _weights(n, k, 5)
+    y = pkg.int8_linear(x, wq, ws, b)
+    for at in (slice(0, 500), slice((1 << 24) - 200, t)):
+        want, tol = ref.product(_np(x[at]), _np(wq), _np(ws), _np(b))
+        _close(y[at], want, tol, torch.float16)
+    h, images = 1 << 13, 1025                  # images of 2 x 8192: the border between the passes lies inside the last but one
+    x = torch.cat([x, x])[:images * 2 * h]
+    z = pkg.int8_conv1x1(x.view(images, 2, h, k).permute(0, 3, 1, 2).contiguous(), wq, ws, b).permute(0, 2, 3, 1).reshape(-1, n)
+    for at in (slice(0, 500), slice((1 << 24) - 500, (1 << 24) + 500), slice(-500, None)):
+        assert torch.equal(z[at], pkg.int8_linear(x[at], wq, ws, b))
