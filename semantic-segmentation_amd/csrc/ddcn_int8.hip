@@ -39,6 +39,13 @@ struct Int8Args {
     int steps_per;                     // K steps of a split
 };
 
+// Workgroups round-robin over the 8 XCDs by launch index: give each XCD a contiguous run of tiles (bijective)
+__device__ __forceinline__ int xcd_logical(int b, int total)
+{
+    const int q = total / 8, r = total % 8, xcd = b % 8, k = b / 8;
+    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + k;
+}
+
 // first element of token t (of the pass) in x
 __device__ __forceinline__ long long token_base(const Int8Args &a, int t)
 {
@@ -135,8 +142,13 @@ template <int DT> __device__ __forceinline__ void load_16(const Int8Args &a, lon
         }
         return;
     }
+    if (k + 16 <= a.k) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = k + e < a.k ? load_one<DT>(a.x, base + (k + e) * a.sk) : 0.f;
+        for (int e = 0; e < 16; ++e) x[e] = load_one<DT>(a.x, base + (k + e) * a.sk);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = k + e < a.k ? load_one<DT>(a.x, base + (k + e) * a.sk) : 0.f;
+    }
 }
 
 // sk == 1: W waves per token, 16 consecutive values per lane and turn, up to I turns held in registers (more are read again)
@@ -146,7 +158,7 @@ template <int DT, int W, int I> __global__ __launch_bounds__(256) void prepare_r
     __shared__ unsigned tops[4];
     constexpr int kTurn = 64 * W;                          // chunks of a turn
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t = blockIdx.x * (4 / W) + wave / W, first = (wave % W) * 64 + lane;
+    const int t = xcd_logical(blockIdx.x, a.prep_blocks) * (4 / W) + wave / W, first = (wave % W) * 64 + lane;
     const bool live = t < a.tokens;
     const long long base = live ? token_base(a, t) : 0;
     constexpr int kAlign = DT == DDCN_F32 ? 4 : 8;
@@ -189,51 +201,116 @@ template <int DT, int W, int I> __global__ __launch_bounds__(256) void prepare_r
     if (first == 0) a.scale[a.q_rows ? a.t0 + t : t] = scale;
 }
 
-// Any strides, lanes along the tokens: 32 tokens per workgroup, half a wave per chunk of 16 channels, I chunks per half
-// wave held in registers (more are read again)
-template <int DT, int NT, int I> __global__ __launch_bounds__(NT) void prepare_map_kernel(const Int8Args a)
+// Sixteen values of a chunk as they are stored: 16-bit ones in pairs
+template <int DT> struct Raw {
+    static constexpr int N = DT == DDCN_F32 ? 16 : 8;
+    unsigned u[N];
+};
+template <int DT> __device__ __forceinline__ Raw<DT> paired(const unsigned (&v)[16])
 {
-    if ((int)blockIdx.x >= a.prep_blocks) return repack_weights(a, blockIdx.x - a.prep_blocks, gridDim.x - a.prep_blocks);
-    constexpr int kHalves = NT / 32;
-    __shared__ unsigned tops[NT / 64][32];
-    const int tl = threadIdx.x & 31, half = threadIdx.x >> 5;
-    const int t = blockIdx.x * 32 + tl;
-    const bool live = t < a.tokens;
-    const long long base = live ? token_base(a, t) : 0;
-    float x[I][16];
-    unsigned top = 0;
-    if (live) {
+    Raw<DT> r;
 #pragma unroll
-        for (int i = 0; i < I; ++i)
-            if (half + i * kHalves < a.chunks) load_16<DT>(a, base, (half + i * kHalves) * 16, false, x[i]);
+    for (int e = 0; e < Raw<DT>::N; ++e) r.u[e] = DT == DDCN_F32 ? v[e] : v[2 * e] | v[2 * e + 1] << 16;
+    return r;
+}
+template <int DT> __device__ __forceinline__ unsigned raw_one(const void *p)
+{
+    return DT == DDCN_F32 ? *(const unsigned *)p : (unsigned)*(const bf16_t *)p;
+}
+// any address and any end of k
+template <int DT> __device__ __forceinline__ Raw<DT> load_raw(const Int8Args &a, long long base, int k)
+{
+    constexpr int kSize = DT == DDCN_F32 ? 4 : 2;
+    unsigned v[16];
 #pragma unroll
-        for (int i = 0; i < I; ++i)
-            if (half + i * kHalves < a.chunks)
+    for (int e = 0; e < 16; ++e) v[e] = k + e < a.k ? raw_one<DT>((const char *)a.x + (base + (k + e) * a.sk) * kSize) : 0u;
+    return paired<DT>(v);
+}
+// `from` is the wave's address of the first value, `off` the lane's distance from it: no address arithmetic per load
+template <int DT> __device__ __forceinline__ Raw<DT> load_raw_near(const char *from, long long step, unsigned off)
+{
+    unsigned v[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = max(top, bits_of(x[i][e]));
-        for (int c = half + I * kHalves; c < a.chunks; c += kHalves) {
-            float z[16];
-            load_16<DT>(a, base, c * 16, false, z);
+    for (int e = 0; e < 16; ++e) v[e] = raw_one<DT>(from + e * step + off);
+    return paired<DT>(v);
+}
+// the larger of `top` and the chunk's magnitudes, on their bits (16-bit formats are ordered by them too, half by half)
+template <int DT> __device__ __forceinline__ unsigned top_raw(const Raw<DT> &r, unsigned top)
+{
+    typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top = max(top, bits_of(z[e]));
+    for (int e = 0; e < Raw<DT>::N; ++e)
+        if (DT == DDCN_F32) top = max(top, r.u[e] & 0x7FFFFFFFu);
+        else top = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), __builtin_bit_cast(u16x2, r.u[e] & 0x7FFF7FFFu)));
+    return top;
+}
+// fp32 bits of what top_raw gives
+template <int DT> __device__ __forceinline__ unsigned top_bits(unsigned top)
+{
+    if (DT == DDCN_F32) return top;
+    const unsigned one = max(top & 0xFFFFu, top >> 16);
+    return DT == DDCN_BF16 ? one << 16 : __float_as_uint(F16::one((bf16_t)one));
+}
+template <int DT> __device__ __forceinline__ u32x4 pack_raw(const Raw<DT> &r, float factor)
+{
+    float x[16];
+#pragma unroll
+    for (int e = 0; e < Raw<DT>::N; ++e) {
+        if (DT == DDCN_F32) x[e] = __uint_as_float(r.u[e]);
+        else {
+            x[2 * e] = DT == DDCN_BF16 ? BF16::lo(r.u[e]) : F16::lo(r.u[e]);
+            x[2 * e + 1] = DT == DDCN_BF16 ? BF16::hi(r.u[e]) : F16::hi(r.u[e]);
         }
     }
-    top = max(top, (unsigned)__shfl_xor((int)top, 32));
-    if ((threadIdx.x & 32) == 0) tops[threadIdx.x >> 6][tl] = top;
-    __syncthreads();
-    for (int w = 0; w < NT / 64; ++w) top = max(top, tops[w][tl]);
-    if (!live) return;
-    float scale, factor;
-    token_scale(top, scale, factor);
+    return pack16(x, factor);
+}
+
+// Any strides, lanes along the tokens: 32 tokens per workgroup; a wave takes two chunks of 16 channels at a time (one per
+// half), I such pairs held in registers as they came (more are read again).  16-bit values in pairs leave room for two
+// workgroups of 1024 on a CU: one loads while the other rounds and stores.
+template <int DT, int NT, int I> __global__ __launch_bounds__(NT, DT != DDCN_F32 && NT == 1024 ? 8 : 4) void prepare_map_kernel(const Int8Args a)
+{
+    if ((int)blockIdx.x >= a.prep_blocks) return repack_weights(a, blockIdx.x - a.prep_blocks, gridDim.x - a.prep_blocks);
+    constexpr int kWaves = NT / 64, kSize = DT == DDCN_F32 ? 4 : 2;
+    __shared__ unsigned tops[kWaves][32];
+    const int tl = threadIdx.x & 31, high = (threadIdx.x >> 5) & 1, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t_first = xcd_logical(blockIdx.x, a.prep_blocks) * 32;    // neighbours share lines of x, and an L2
+    const int t = t_first + tl;
+    const bool live = t < a.tokens;
+    const long long start = token_base(a, t_first), base = live ? token_base(a, t) : start;
+    // the lane's distance from the workgroup's first token, with the half's 16 channels: within 32 bits nearly always
+    const long long apart = (base - start + high * 16 * a.sk) * kSize;
+    const bool near = __all(apart >= 0 && apart < (1LL << 31));
+    const char *from = (const char *)a.x + start * kSize;
+    auto load = [&](int pair) {
+        if (near && (pair + 1) * 32 <= a.k) return load_raw_near<DT>(from + pair * 32 * a.sk * kSize, a.sk * kSize, (unsigned)apart);
+        return load_raw<DT>(a, base, (pair * 2 + high) * 16);
+    };
+    const int pairs = (a.chunks + 1) / 2;
+    Raw<DT> x[I];
+    unsigned top = 0;
 #pragma unroll
     for (int i = 0; i < I; ++i)
-        if (half + i * kHalves < a.chunks) store_chunk(a, t, half + i * kHalves, pack16(x[i], factor));
-    for (int c = half + I * kHalves; c < a.chunks; c += kHalves) {
-        float z[16];
-        load_16<DT>(a, base, c * 16, false, z);
-        store_chunk(a, t, c, pack16(z, factor));
-    }
-    if (half == 0) a.scale[a.q_rows ? a.t0 + t : t] = scale;
+        if (wave + i * kWaves < pairs) x[i] = load(wave + i * kWaves);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+        if (wave + i * kWaves < pairs) top = top_raw<DT>(x[i], top);
+    for (int p = wave + I * kWaves; p < pairs; p += kWaves) top = top_raw<DT>(load(p), top);
+    top = top_bits<DT>(top);
+    top = max(top, (unsigned)__shfl_xor((int)top, 32));
+    if (high == 0) tops[wave][tl] = top;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) top = max(top, tops[w][tl]);
+    float scale, factor;
+    token_scale(top, scale, factor);
+    auto store = [&](int pair, const Raw<DT> &r) {
+        if (live && pair * 2 + high < a.chunks) store_chunk(a, t, pair * 2 + high, pack_raw<DT>(r, factor));
+    };
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+        if (wave + i * kWaves < pairs) store(wave + i * kWaves, x[i]);
+    for (int p = wave + I * kWaves; p < pairs; p += kWaves) store(p, load(p));
+    if (live && wave == 0 && high == 0) a.scale[a.q_rows ? a.t0 + t : t] = scale;
 }
 
 // ---------------------------------------------------------------- epilogue
@@ -254,13 +331,6 @@ template <bool NCHW> __device__ __forceinline__ long long out_base(const Int8Arg
 }
 
 // ---------------------------------------------------------------- product
-// Workgroups round-robin over the 8 XCDs by launch index: give each XCD a contiguous run of tiles (bijective)
-__device__ __forceinline__ int xcd_logical(int b, int total)
-{
-    const int q = total / 8, r = total % 8, xcd = b % 8, k = b / 8;
-    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + k;
-}
-
 // N requests of 16 bytes per lane from `from` (`bytes` readable there), to LDS STEP bytes apart
 template <int N, int STEP> __device__ __forceinline__ void dma(const u32x4 *from, unsigned bytes, char *to, const unsigned *off)
 {
@@ -275,33 +345,65 @@ __device__ __forceinline__ i32x4 mfma8(u32x4 a, u32x4 b, i32x4 c)
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
-// Rows of the tile run along the registers of the result, columns along its lanes; the columns are what is contiguous in y:
-// tokens for nchw (rows: channels), channels otherwise (rows: tokens).  Tile 2*MI*32 rows x 64*NWN columns, 2 x NWN waves of
-// MI*32 x 64.  A ring of NS K steps (64 k each) in LDS, filled by DMA: request of step s + NS goes into the stage that step s
-// has left.  One barrier per step, between the two halves of its MFMAs: fragments are read one half ahead of their use.
+// Rows of the tile run along the registers of the result, columns along its lanes; the rows are what is contiguous in y --
+// tokens for nchw (columns: channels), channels otherwise (columns: tokens) -- so that a lane ends with runs of y in its
+// registers and stores 16 bytes at a time (stores of single 16-bit elements cost 65 cycles each: 28 us of a 256-tile round).
+// For that, LDS slot s of a 32-row group holds row `row_of(s)`: a lane's results of two neighbouring 16-row tiles are then
+// eight consecutive rows (16-bit results; four of one tile for fp32).
+// Tile 2*MI*32 rows x 64*NWN columns, 2 x NWN waves of MI*32 x 64.  A ring of NS K steps (64 k each) in LDS, filled by DMA:
+// the request of step s + NS goes into the stage that step s has left.  One barrier per step, between the two halves of its
+// MFMAs: fragments are read one half ahead of their use.
+template <bool PAIRS> __device__ __forceinline__ int row_of(int s)
+{
+    // slot = tile * 16 + quad * 4 + e  ->  row = quad * 8 + tile * 4 + e
+    return PAIRS ? (s & ~31) | ((s >> 2) & 3) << 3 | ((s >> 4) & 1) << 2 | (s & 3) : s;
+}
+
+// N consecutive values of y; the address is aligned to its elements only
+template <int DT, int N> __device__ __forceinline__ void store_run(void *y, long long at, const float (&v)[N])
+{
+    if (DT == DDCN_F32) {
+        struct __attribute__((packed, aligned(4))) Run {
+            float f[N];
+        } r;
+#pragma unroll
+        for (int e = 0; e < N; ++e) r.f[e] = v[e];
+        *(Run *)((float *)y + at) = r;
+    } else {
+        struct __attribute__((packed, aligned(2))) Run {
+            unsigned u[N / 2];
+        } r;
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e)
+            r.u[e] = DT == DDCN_BF16 ? BF16::pack2(v[2 * e], v[2 * e + 1]) : F16::pack2(v[2 * e], v[2 * e + 1]);
+        *(Run *)((bf16_t *)y + at) = r;
+    }
+}
+
 template <int DT, bool NCHW, bool PART, int MI, int NWN, int NS>
-__global__ __launch_bounds__(128 * NWN, NWN == 4 ? 1 : 2) void gemm8_kernel(const Int8Args a)
+__global__ __launch_bounds__(128 * NWN, 4) void gemm8_kernel(const Int8Args a)
 {
     constexpr int NT = 128 * NWN, NWAVES = NT / 64, BR = 2 * MI * 32, BC = 64 * NWN;
     constexpr int RR = BR * 4 / NT, RC = BC * 4 / NT;      // requests per thread and step
     constexpr int STAGE = BR * 4 + BC * 4;                 // 16-byte chunks of a stage
+    constexpr bool PAIRS = !PART && DT != DDCN_F32;
     extern __shared__ u32x4 ring[];
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wr = wave / NWN, wc = wave % NWN;
-    const int rows = NCHW ? a.channels : a.tokens, cols = NCHW ? a.tokens : a.channels;
-    const u32x4 *R = NCHW ? a.wp : a.q, *C = NCHW ? a.q : a.wp;
-    const long long ldr = NCHW ? a.channels : a.ldq, ldc = NCHW ? a.ldq : a.channels;
+    const int rows = NCHW ? a.tokens : a.channels, cols = NCHW ? a.channels : a.tokens;
+    const u32x4 *R = NCHW ? a.q : a.wp, *C = NCHW ? a.wp : a.q;
+    const long long ldr = NCHW ? a.ldq : a.channels, ldc = NCHW ? a.channels : a.ldq;
     const int tiles_r = (rows + BR - 1) / BR, tiles_c = (cols + BC - 1) / BC;
     const int L = xcd_logical(blockIdx.x, tiles_r * tiles_c);
     // neighbours share the tile of tokens, the larger operand
-    const int r0 = (NCHW ? L % tiles_r : L / tiles_c) * BR, c0 = (NCHW ? L / tiles_r : L % tiles_c) * BC;
+    const int r0 = (NCHW ? L / tiles_c : L % tiles_r) * BR, c0 = (NCHW ? L % tiles_c : L / tiles_r) * BC;
     const int first = blockIdx.y * a.steps_per, steps = min(a.steps_per, a.chunks / 4 - first);
 
     unsigned off_r[RR], off_c[RC];
 #pragma unroll
     for (int i = 0; i < RR; ++i) {
-        const int q = (i * NWAVES + wave) * 64 + lane, row = q % BR;
+        const int q = (i * NWAVES + wave) * 64 + lane, row = row_of<PAIRS>(q % BR);
         off_r[i] = r0 + row < rows ? (unsigned)((q / BR) * ldr + row) * 16u : DMA_OOB;
     }
 #pragma unroll
@@ -338,12 +440,11 @@ __global__ __launch_bounds__(128 * NWN, NWN == 4 ? 1 : 2) void gemm8_kernel(cons
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc[h * MI + i][j] = mfma8(fr[i], fc[j], acc[h * MI + i][j]);
+            for (int j = 0; j < 4; ++j) acc[h * MI + i][j] = mfma8(fr[i], fc[j], acc[h * MI + i][j]);
     };
     // this wave's LDS reads are done and all but its `younger` youngest steps have landed
     auto wait_but = [&](int younger) {
-        if (younger >= 3) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(3 * (RR + RC)));
+        if (NS > 3 && younger >= 3) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(3 * (RR + RC)));
         else if (younger == 2) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(2 * (RR + RC)));
         else if (younger == 1) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(RR + RC));
         else __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
@@ -381,55 +482,114 @@ __global__ __launch_bounds__(128 * NWN, NWN == 4 ? 1 : 2) void gemm8_kernel(cons
         if (s + 1 < steps) step(s + 1, fy, fx);
     }
 
-    // lane l holds rows 4 * (l / 16) + e, column l % 16 of each 16 x 16 tile
-    const int row0 = r0 + wr * (MI * 32) + kc * 4, col0 = c0 + wc * 64 + r16;
+    // lane l holds slots 4 * (l / 16) + e, column l % 16 of each 16 x 16 tile: runs of N consecutive rows
+    constexpr int N = PAIRS ? 8 : 4, T = N / 4;
+    const int row0 = r0 + wr * (MI * 32) + kc * N, col0 = c0 + wc * 64 + r16;
+    float sc[4], bc[4];
+    if (!PART)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int col = min(col0 + j * 16, cols - 1);
+            sc[j] = NCHW ? a.w_scale[col] : a.scale[col];
+            bc[j] = NCHW && a.bias ? a.bias[col] : 0.f;
+        }
     if (PART) {
-        int *part = a.part + (long long)blockIdx.y * rows * cols;
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < RT; ++i) {
+            const int row = row0 + i * 16, live = min(rows - row, 4);
+            int *part = a.part + (long long)blockIdx.y * rows * cols + row;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = row0 + i * 16 + e;
+            for (int j = 0; j < 4; ++j) {
+                const int col = col0 + j * 16;
+                if (col >= cols || live <= 0) continue;
+                int *to = part + (long long)col * rows;
+                if (live == 4 && (rows & 3) == 0) *(i32x4 *)to = acc[i][j];
+                else
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (row < rows && col0 + j * 16 < cols) part[(long long)row * cols + col0 + j * 16] = acc[i][j][e];
+                    for (int e = 0; e < 4; ++e)
+                        if (e < live) to[e] = acc[i][j][e];
             }
+        }
         return;
     }
-    float sc[4], bc[4];
-    long long at[4];
+    constexpr int G = RT / T;                              // runs of a lane and column
+    float sr[G][N], br[G][N];
+    long long base[G];                                     // the run's place in y, without its column
+    unsigned place[G];                                     // and in its image (nchw)
+    bool whole[G];                                         // all of it exists, in one image
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int col = min(col0 + j * 16, cols - 1);
-        sc[j] = NCHW ? a.scale[col] : a.w_scale[col];
-        bc[j] = !NCHW && a.bias ? a.bias[col] : 0.f;
-        at[j] = NCHW ? out_base<true>(a, col) : col;
+    for (int g = 0; g < G; ++g) {
+        const int row = row0 + g * T * 16;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int at = min(row + e, rows - 1);
+            sr[g][e] = NCHW ? a.scale[at] : a.w_scale[at];
+            br[g][e] = !NCHW && a.bias ? a.bias[at] : 0.f;
+        }
+        const unsigned u = (unsigned)(a.t0 + row), img = NCHW ? u / (unsigned)a.plane : 0u;
+        place[g] = NCHW ? u - img * (unsigned)a.plane : 0u;
+        whole[g] = rows - row >= N && (!NCHW || place[g] + N <= (unsigned)a.plane);
+        base[g] = NCHW ? (long long)img * a.channels * a.plane + place[g] : row;
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int j = 0; j < 4; ++j) {
+        const int col = col0 + j * 16;
+        const bool exists = col < cols;
+        const long long off = NCHW ? (long long)col * a.plane : (a.t0 + col) * (long long)a.channels;
+        float v[G][N];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = row0 + i * 16 + e;
-            if (row >= rows) continue;
-            const float sr = NCHW ? a.w_scale[row] : a.scale[row], br = NCHW && a.bias ? a.bias[row] : 0.f;
-            const long long ro = NCHW ? (long long)row * a.plane : out_base<false>(a, row);
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col0 + j * 16 < cols)
-                    store_one<DT>(a.y, ro + at[j], finished(a, acc[i][j][e], NCHW ? sc[j] : sr, NCHW ? sr : sc[j], NCHW ? br : bc[j]));
+            for (int e = 0; e < N; ++e)
+                v[g][e] = finished(a, acc[g * T + e / 4][j][e & 3], NCHW ? sr[g][e] : sc[j], NCHW ? sc[j] : sr[g][e], NCHW ? bc[j] : br[g][e]);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int row = row0 + g * T * 16, live = rows - row;
+            const long long at = base[g] + off;
+            // A 16-byte store at an odd address (in 16-bit elements: every other channel of a map with an odd number of
+            // pixels) takes twice as long as one at an even one.  There a run is written one element on: its own 1 .. 7 and
+            // the first of the next run, which the lane 16 on holds (from the fourth sixteen on: the first sixteen's, of
+            // the next g).  Its own first element is written by the run before it, where there is one in the wave and image.
+            bool odd = false;
+            if (PAIRS) {
+                odd = exists && whole[g] && (((unsigned long long)a.y >> 1) + at & 1) != 0;
+                if (__any(odd)) {
+                    const float give = kc == 0 ? v[g + 1 < G ? g + 1 : g][0] : v[g][0];
+                    const float next = __shfl(give, (lane + 16) & 63);
+                    const bool more = !(g == G - 1 && kc == 3) && live > N && place[g] + N < (unsigned)(NCHW ? a.plane : 0x7fffffff);
+                    if (odd) {
+                        if ((g == 0 && kc == 0) || (NCHW && place[g] < N)) store_one<DT>(a.y, at, v[g][0]);
+                        if (more) {
+                            const float r[8] = {v[g][1], v[g][2], v[g][3], v[g][N > 4 ? 4 : 0], v[g][N > 4 ? 5 : 0], v[g][N > 4 ? 6 : 0], v[g][N > 4 ? 7 : 0], next};
+                            store_run<DT, 8>(a.y, at + 1, r);
+                        } else {
+                            const float r[6] = {v[g][1], v[g][2], v[g][3], v[g][N > 4 ? 4 : 0], v[g][N > 4 ? 5 : 0], v[g][N > 4 ? 6 : 0]};
+                            store_run<DT, 6>(a.y, at + 1, r);
+                            store_one<DT>(a.y, at + 7, v[g][N > 4 ? 7 : 0]);
+                        }
+                    }
+                }
+            }
+            if (!exists || odd || live <= 0) continue;
+            if (whole[g]) store_run<DT, N>(a.y, at, v[g]);
+            else
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (e < live) store_one<DT>(a.y, NCHW ? out_base<true>(a, row + e) + off : at + e, v[g][e]);
         }
+    }
 }
 
-// sums [split][rows][cols] -> y
+// sums [split][columns][rows] -> y, in the order of y
 template <int DT, bool NCHW> __global__ __launch_bounds__(256) void finish_kernel(const Int8Args a, int splits)
 {
-    const int rows = NCHW ? a.channels : a.tokens, cols = NCHW ? a.tokens : a.channels;
+    const int rows = NCHW ? a.tokens : a.channels, cols = NCHW ? a.channels : a.tokens;
     const long long total = (long long)rows * cols, i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
     int sum = 0;
     for (int s = 0; s < splits; ++s) sum += a.part[s * total + i];
-    const int row = (int)(i / cols), col = (int)(i - (long long)row * cols);
-    const int tok = NCHW ? col : row, n = NCHW ? row : col;
+    const int col = (int)(i / rows), row = (int)(i - (long long)col * rows);
+    const int tok = NCHW ? row : col, n = NCHW ? col : row;
     store_one<DT>(a.y, out_base<NCHW>(a, tok) + (NCHW ? (long long)n * a.plane : n),
                   finished(a, sum, a.scale[tok], a.w_scale[n], a.bias ? a.bias[n] : 0.f));
 }
@@ -490,7 +650,7 @@ long long tokens_of(const ddcn_int8_geom *g) { return (long long)g->images * g->
 // How a pass of `tokens` tokens is computed
 struct Plan {
     bool gemv;
-    int tile;              // 0: 256 x 256, 1: 128 x 128, 2: 64 x 64
+    bool small;            // tiles of 64 x 64 instead of 128 x 128
     int splits, steps_per;
     size_t q_bytes, scale_bytes, w_bytes, part_bytes;
     size_t bytes() const { return q_bytes + scale_bytes + w_bytes + part_bytes; }
@@ -508,12 +668,11 @@ Plan plan_of(const ddcn_int8_geom *g, long long tokens)
     p.gemv = tokens <= kGemvTokens;
     if (p.gemv) return p;
     p.w_bytes = round_up((size_t)(chunks * 16 * g->channels), 256);
-    const long long sizes[3] = {256, 128, 64};
-    long long tiles = 0;
-    for (p.tile = 0; p.tile < 3; ++p.tile) {
-        tiles = ceil_div(tokens, sizes[p.tile]) * ceil_div(g->channels, sizes[p.tile]);
-        if (tiles >= kCUs * 3 / 4 || p.tile == 2) break;
-    }
+    // 128 x 128 tiles, four workgroups on a CU: 18818 x 2048 x 512 takes 28 us, 32768 x 2048 x 512 37 us (256 x 256 with
+    // one workgroup on a CU: 52 and 39; 256 x 128: 35 and 40).  Smaller ones where those leave a quarter of the CUs idle.
+    long long tiles = ceil_div(tokens, 128) * ceil_div(g->channels, 128);
+    p.small = tiles < kCUs * 3 / 4;
+    if (p.small) tiles = ceil_div(tokens, 64) * ceil_div(g->channels, 64);
     // K is split where the tiles leave CUs without work, into pieces of 8 steps at least
     long long splits = tiles >= kCUs ? 1 : ceil_div(2 * kCUs, tiles);
     if (splits > steps / 8) splits = steps / 8 > 1 ? steps / 8 : 1;
@@ -556,14 +715,13 @@ template <int DT, bool NCHW, bool PART, int MI, int NWN, int NS> int launch_tile
     constexpr int BR = 2 * MI * 32, BC = 64 * NWN, kLds = NS * (BR + BC) * 64;
     static std::atomic<uint64_t> done{0};
     if (!raise_lds_limit((const void *)gemm8_kernel<DT, NCHW, PART, MI, NWN, NS>, kLds, done)) return fail(DDCN_ERR_LAUNCH, "int8 product: LDS limit");
-    const long long rows = NCHW ? a.channels : a.tokens, cols = NCHW ? a.tokens : a.channels;
+    const long long rows = NCHW ? a.tokens : a.channels, cols = NCHW ? a.channels : a.tokens;
     gemm8_kernel<DT, NCHW, PART, MI, NWN, NS><<<dim3((unsigned)(ceil_div(rows, BR) * ceil_div(cols, BC)), (unsigned)splits), 128 * NWN, kLds, s>>>(a);
     return check_launch("int8 product");
 }
 template <int DT, bool NCHW, bool PART> int launch_gemm(const Int8Args &a, const Plan &p, hipStream_t s)
 {
-    if (p.tile == 0) return launch_tiles<DT, NCHW, PART, 4, 4, 4>(a, p.splits, s);
-    if (p.tile == 1) return launch_tiles<DT, NCHW, PART, 2, 2, 4>(a, p.splits, s);
+    if (!p.small) return launch_tiles<DT, NCHW, PART, 2, 2, 2>(a, p.splits, s);
     return launch_tiles<DT, NCHW, PART, 1, 1, 4>(a, p.splits, s);
 }
 template <int DT, bool NCHW> int launch_product(const Int8Args &a, const Plan &p, hipStream_t s)
