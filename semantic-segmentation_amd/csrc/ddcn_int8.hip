@@ -2,9 +2,10 @@
 // stand in include/ddcn_hip.h.
 //
 //   prepare_*    x (any strides) -> codes and the tokens' scales; workgroups behind those of the tokens repack the weights
-//   gemm8        codes x weights on v_mfma_i32_16x16x64_i8, operands global -> LDS by DMA through a ring of K steps; exact
+//   gemm8        (more than 512 tokens) codes x weights on v_mfma_i32_16x16x64_i8, operands global -> LDS by DMA through a ring of K steps; exact
 //                int32 sums, scales + bias + ReLU in the epilogue, or int32 partial sums where K is split
-//   gemv8        up to 16 tokens: a wave per channel streams its weights once, v_dot4_i32_i8
+//   direct8      (17 to 512 tokens) both operands straight into the MFMA's registers, weights from the caller's rows
+//   gemv8        (up to 16) a wave per channel streams its weights once, v_dot4_i32_i8; up to 4 tokens it rounds them too
 //   finish       sums of the partial sums, epilogue
 //
 // Codes and repacked weights are stored as [k / 16][token or channel][16]: sixteen consecutive k of one row are one operand
@@ -36,7 +37,7 @@ struct Int8Args {
     int plane, cols;                   // of an image
     int k, chunks, channels, relu;     // chunks: of 16 k, whole K steps
     int prep_blocks;                   // workgroups of the tokens; the rest repack weights
-    int steps_per;                     // K steps of a split
+    int splits, steps_per;             // of K, and K steps of one
 };
 
 // Workgroups round-robin over the 8 XCDs by launch index: give each XCD a contiguous run of tiles (bijective)
@@ -87,6 +88,7 @@ __device__ __forceinline__ u32x4 pack16(const float (&x)[16], float factor)
 // 16 weight bytes from k on, zero behind the row's kk bytes
 __device__ __forceinline__ u32x4 weight_chunk(const signed char *row, int k, int kk, bool wide)
 {
+    if (k >= kk) return u32x4{0u, 0u, 0u, 0u};
     if (wide && k + 16 <= kk) return *(const u32x4 *)(row + k);
     unsigned u[4] = {0u, 0u, 0u, 0u};
     for (int e = 0; e < 16; ++e)
@@ -395,10 +397,11 @@ __global__ __launch_bounds__(128 * NWN, 4) void gemm8_kernel(const Int8Args a)
     const u32x4 *R = NCHW ? a.q : a.wp, *C = NCHW ? a.wp : a.q;
     const long long ldr = NCHW ? a.ldq : a.channels, ldc = NCHW ? a.channels : a.ldq;
     const int tiles_r = (rows + BR - 1) / BR, tiles_c = (cols + BC - 1) / BC;
-    const int L = xcd_logical(blockIdx.x, tiles_r * tiles_c);
-    // neighbours share the tile of tokens, the larger operand
+    // Whole K: neighbours share the tile of tokens, the larger operand.  Split: an XCD takes one piece of K (the splits are
+    // mostly a power of two) and its L2 reads that piece of both operands alone.
+    const int L = PART ? blockIdx.x / a.splits : xcd_logical(blockIdx.x, tiles_r * tiles_c), split = PART ? blockIdx.x % a.splits : 0;
     const int r0 = (NCHW ? L / tiles_c : L % tiles_r) * BR, c0 = (NCHW ? L % tiles_c : L / tiles_r) * BC;
-    const int first = blockIdx.y * a.steps_per, steps = min(a.steps_per, a.chunks / 4 - first);
+    const int first = split * a.steps_per, steps = min(a.steps_per, a.chunks / 4 - first);
 
     unsigned off_r[RR], off_c[RC];
 #pragma unroll
@@ -497,7 +500,7 @@ __global__ __launch_bounds__(128 * NWN, 4) void gemm8_kernel(const Int8Args a)
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             const int row = row0 + i * 16, live = min(rows - row, 4);
-            int *part = a.part + (long long)blockIdx.y * rows * cols + row;
+            int *part = a.part + (long long)split * rows * cols + row;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int col = col0 + j * 16;
@@ -595,35 +598,211 @@ template <int DT, bool NCHW> __global__ __launch_bounds__(256) void finish_kerne
 }
 
 // ---------------------------------------------------------------- few tokens
-// A wave per channel, TOK tokens: the weights are read once, straight from the caller's rows, 16 bytes per lane and turn;
-// the codes of a chunk lie next to each other and come from the caches.
-template <int DT, bool NCHW, int TOK> __global__ __launch_bounds__(256) void gemv8_kernel(const Int8Args a)
+// Up to kDirectTokens (512 x 2048 x 512: 8.2 us, tiles with split K 6.4 + 3.1 and the repacking of the weights; 300 x 12544 x
+// 1024: 22.5, tiles 15.5 + 4.3 + 3; above, tiles win): what counts is to stream the weights once, from the caller's own rows (repacking them moves as many
+// bytes again, twice).  64 tokens x 32 channels per workgroup, K dealt to its eight waves in turns of 128 k (a
+// line of a weight row); both operands go
+// straight into the MFMA's registers (a weight fragment is 16 rows x 64 bytes, a code fragment four runs of 256), two
+// turns ahead, and nothing is shared until the waves' sums meet in LDS.
+template <int DT, bool NCHW> __global__ __launch_bounds__(512) void direct8_kernel(const Int8Args a)
 {
-    const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= a.channels) return;
+    constexpr bool PAIRS = DT != DDCN_F32;
+    constexpr int NR = NCHW ? 4 : 2, NC = NCHW ? 2 : 4;    // tiles of 16 rows (registers, contiguous in y) and columns (lanes)
+    constexpr int kWaves = 8, kAhead = 2;
+    __shared__ i32x4 sums[kWaves][NR * NC][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kc = lane >> 4;
+    // an XCD takes a range of channels and all tokens: its L2 then reads its part of the weights alone
+    const int across = (a.tokens + 63) / 64, L = xcd_logical(blockIdx.x, gridDim.x);
+    const int t0 = L % across * 64, n0 = L / across * 32;
+    const int rows = NCHW ? a.tokens : a.channels, cols = NCHW ? a.channels : a.tokens;
+    const int r0 = NCHW ? t0 : n0, c0 = NCHW ? n0 : t0;
+    // this lane's tokens and weight rows (clamped: what is computed for the others is not stored)
+    const u32x4 *qp[4];
+    const signed char *wp[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) qp[i] = a.q + min(t0 + (NCHW ? row_of<PAIRS>(i * 16 + r16) : i * 16 + r16), a.tokens - 1) + kc * a.ldq;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) wp[i] = a.w + min(n0 + (NCHW ? i * 16 + r16 : row_of<PAIRS>(i * 16 + r16)), a.channels - 1) * a.ldw + kc * 16;
+    struct Frags {
+        u32x4 q[2][4], w[2][2];
+    };
+    const int full = a.k / 128;                            // turns whose weights need no guard
+    auto load = [&](int s) {
+        Frags f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) f.w[h][i] = *(const u32x4 *)(wp[i] + s * 128 + h * 64);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f.q[h][i] = qp[i][((long long)s * 8 + h * 4) * a.ldq];
+        return f;
+    };
+    i32x4 acc[NR][NC];
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    auto mul = [&](const Frags &f) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+#pragma unroll
+                for (int j = 0; j < NC; ++j) acc[i][j] = NCHW ? mfma8(f.q[h][i], f.w[h][j & 1], acc[i][j]) : mfma8(f.w[h][i & 1], f.q[h][j], acc[i][j]);
+    };
+    Frags f[kAhead];
+    int s = wave;
+    // while the next kAhead turns exist, every turn loads one: the number of loads in flight is known, and a turn waits for
+    // its own alone
+    if (s + (2 * kAhead - 1) * kWaves < full) {
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) f[d] = load(s + d * kWaves);
+        for (; s + (2 * kAhead - 1) * kWaves < full; s += kAhead * kWaves)
+#pragma unroll
+            for (int d = 0; d < kAhead; ++d) {
+                mul(f[d]);
+                f[d] = load(s + (d + kAhead) * kWaves);
+            }
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) mul(f[d]);
+        s += kAhead * kWaves;
+    }
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d)
+        if (s + d * kWaves < full) f[d] = load(s + d * kWaves);
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d)
+        if (s + d * kWaves < full) mul(f[d]);
+    s += kAhead * kWaves;
+    for (; s < full; s += kWaves) mul(load(s));
+    if (full * 128 < a.k && wave == full % kWaves) {       // the end of K; the codes are padded with zeros to whole 64
+        Frags e;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = full * 128 + h * 64;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) e.w[h][i] = weight_chunk(wp[i] - kc * 16, k + kc * 16, a.k, true);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e.q[h][i] = k < a.k ? qp[i][(long long)(k / 16) * a.ldq] : u32x4{0u, 0u, 0u, 0u};
+        }
+        mul(e);
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) sums[wave][i * NC + j][lane] = acc[i][j];
+    __syncthreads();
+    // a wave finishes one pair of row tiles and one column tile: four of them, the other waves are done
+    constexpr int T = 2, kParts = NR / T * NC;
+    static_assert(kParts == 4, "64 x 32");
+    if (wave >= kParts) return;
+    const int i0 = wave / NC * T, j = wave % NC;
+    int v[T][4] = {};
+    for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+        for (int i = 0; i < T; ++i) {
+            const i32x4 p = sums[w][(i0 + i) * NC + j][lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] += p[e];
+        }
+    const int col = c0 + j * 16 + r16;
+    if (col >= cols) return;
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = r0 + i0 * 16 + (PAIRS ? kc * 8 + i * 4 + e : i * 16 + kc * 4 + e);
+            if (row >= rows) continue;
+            const int t = NCHW ? row : col, n = NCHW ? col : row;
+            store_one<DT>(a.y, out_base<NCHW>(a, t) + (NCHW ? (long long)n * a.plane : n),
+                          finished(a, v[i][e], a.scale[t], a.w_scale[n], a.bias ? a.bias[n] : 0.f));
+        }
+}
+
+// Up to 16 tokens: a wave per channel, the weights read once, straight from the caller's rows, 16 bytes per lane and turn;
+// the codes of a chunk lie next to each other.  FUSED (up to TOK = 4 tokens whose codes fit LDS): every workgroup rounds the
+// tokens itself while its first weights are on their way -- one launch, no workspace; the rounding is repeated by every
+// workgroup, from the caches.
+template <int DT, int IN, bool NCHW, int TOK, bool FUSED> __global__ __launch_bounds__(256) void gemv8_kernel(const Int8Args a)
+{
+    extern __shared__ u32x4 codes[];                       // FUSED: [chunk][TOK]
+    __shared__ unsigned tops[4][TOK];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = min((int)blockIdx.x * 4 + wave, a.channels - 1);
     const bool wide = wide_rows(a);
     const signed char *row = a.w + n * a.ldw;
-    int acc[TOK] = {};
-#pragma unroll 4
-    for (int c = lane; c < a.chunks; c += 64) {
-        const u32x4 w = weight_chunk(row, c * 16, a.k, wide);
+    constexpr int kAhead = 4;
+    const int full = wide ? a.k / 16 : 0;                  // chunks that one wide load brings
+    u32x4 ahead[kAhead];
+    auto weights = [&](int c) { return *(const u32x4 *)(row + min(c, full - 1) * 16); };
+    if (full)
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) ahead[d] = weights(lane + 64 * d);
+    float scale[TOK];
+    if (FUSED) {
+        constexpr int kAlign = IN == DDCN_F32 ? 4 : 8;
 #pragma unroll
         for (int t = 0; t < TOK; ++t) {
-            const u32x4 q = a.q[(long long)c * a.ldq + min(t, a.tokens - 1)];
+            const long long base = token_base(a, min(t, a.tokens - 1));
+            const bool vec = a.sk == 1 && (base & (kAlign - 1)) == 0 && ((unsigned long long)a.x & 15) == 0;
+            unsigned top = 0;
+            for (int c = threadIdx.x; c < a.chunks; c += 256) {
+                float x[16];
+                load_16<IN>(a, base, c * 16, vec, x);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = max(top, bits_of(x[e]));
+            }
+            for (int d = 32; d; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
+            if (lane == 0) tops[wave][t] = top;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < TOK; ++t) {
+            const long long base = token_base(a, min(t, a.tokens - 1));
+            const bool vec = a.sk == 1 && (base & (kAlign - 1)) == 0 && ((unsigned long long)a.x & 15) == 0;
+            float factor;
+            token_scale(max(max(tops[0][t], tops[1][t]), max(tops[2][t], tops[3][t])), scale[t], factor);
+            for (int c = threadIdx.x; c < a.chunks; c += 256) {
+                float x[16];
+                load_16<IN>(a, base, c * 16, vec, x);
+                codes[c * TOK + t] = pack16(x, factor);
+            }
+        }
+        __syncthreads();
+    }
+    int acc[TOK] = {};
+    auto dot = [&](int c, u32x4 w) {
+#pragma unroll
+        for (int t = 0; t < TOK; ++t) {
+            const u32x4 q = FUSED ? codes[c * TOK + t] : a.q[(long long)c * a.ldq + min(t, a.tokens - 1)];
 #pragma unroll
             for (int d = 0; d < 4; ++d) acc[t] = __builtin_amdgcn_sdot4((int)w[d], (int)q[d], acc[t], false);
         }
+    };
+    for (int c0 = 0; c0 < full; c0 += 64 * kAhead) {       // (a wave's lanes stay together: every turn loads)
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) {
+            const int c = c0 + 64 * d + lane;
+            if (c < full) dot(c, ahead[d]);
+            ahead[d] = weights(c + 64 * kAhead);
+        }
     }
+    for (int c = full + lane; c * 16 < a.k; c += 64) dot(c, weight_chunk(row, c * 16, a.k, wide));
 #pragma unroll
     for (int t = 0; t < TOK; ++t)
         for (int d = 32; d; d >>= 1) acc[t] += __shfl_xor(acc[t], d);
     // lane t writes token t
     int sum = acc[0];
+    float st = FUSED ? scale[0] : a.scale[min(lane, a.tokens - 1)];
 #pragma unroll
-    for (int t = 1; t < TOK; ++t) sum = lane == t ? acc[t] : sum;
-    if (lane >= a.tokens) return;
+    for (int t = 1; t < TOK; ++t) {
+        sum = lane == t ? acc[t] : sum;
+        if (FUSED) st = lane == t ? scale[t] : st;
+    }
+    if (lane >= a.tokens || (int)blockIdx.x * 4 + wave >= a.channels) return;
     store_one<DT>(a.y, out_base<NCHW>(a, lane) + (NCHW ? (long long)n * a.plane : n),
-                  finished(a, sum, a.scale[lane], a.w_scale[n], a.bias ? a.bias[n] : 0.f));
+                  finished(a, sum, st, a.w_scale[n], a.bias ? a.bias[n] : 0.f));
 }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -649,7 +828,7 @@ long long tokens_of(const ddcn_int8_geom *g) { return (long long)g->images * g->
 
 // How a pass of `tokens` tokens is computed
 struct Plan {
-    bool gemv;
+    int how;               // kFused, kGemv, kDirect, kTiles
     bool small;            // tiles of 64 x 64 instead of 128 x 128
     int splits, steps_per;
     size_t q_bytes, scale_bytes, w_bytes, part_bytes;
@@ -657,25 +836,36 @@ struct Plan {
 };
 
 constexpr int kCUs = 256;
-constexpr int kGemvTokens = 16;
+constexpr int kFusedTokens = 4, kGemvTokens = 16, kDirectTokens = 512;
+constexpr size_t kFusedLds = 64512;       // with the maxima within the 64 KiB that need no attribute
+enum { kFused, kGemv, kDirect, kTiles };
 
-Plan plan_of(const ddcn_int8_geom *g, long long tokens)
+// wide: the weights' rows start on 16 bytes (the sizes are the same either way)
+Plan plan_of(const ddcn_int8_geom *g, long long tokens, bool wide)
 {
     Plan p = {};
     const long long chunks = ceil_div(g->k, 64) * 4, steps = chunks / 4;
     p.q_bytes = round_up((size_t)(chunks * 16 * tokens), 256);
     p.scale_bytes = round_up((size_t)tokens * sizeof(float), 256);
-    p.gemv = tokens <= kGemvTokens;
-    if (p.gemv) return p;
+    const int tok = tokens == 1 ? 1 : kFusedTokens;
+    if (tokens <= kFusedTokens && (size_t)(chunks * 16 * tok) <= kFusedLds) {
+        p.how = kFused;
+        p.q_bytes = p.scale_bytes = 0;
+        return p;
+    }
+    p.how = tokens <= kGemvTokens ? kGemv : tokens <= kDirectTokens && wide ? kDirect : kTiles;
+    if (p.how == kGemv) return p;
     p.w_bytes = round_up((size_t)(chunks * 16 * g->channels), 256);
     // 128 x 128 tiles, four workgroups on a CU: 18818 x 2048 x 512 takes 28 us, 32768 x 2048 x 512 37 us (256 x 256 with
     // one workgroup on a CU: 52 and 39; 256 x 128: 35 and 40).  Smaller ones where those leave a quarter of the CUs idle.
     long long tiles = ceil_div(tokens, 128) * ceil_div(g->channels, 128);
     p.small = tiles < kCUs * 3 / 4;
     if (p.small) tiles = ceil_div(tokens, 64) * ceil_div(g->channels, 64);
-    // K is split where the tiles leave CUs without work, into pieces of 8 steps at least
-    long long splits = tiles >= kCUs ? 1 : ceil_div(2 * kCUs, tiles);
-    if (splits > steps / 8) splits = steps / 8 > 1 ? steps / 8 : 1;
+    // K is split where the tiles leave CUs without work, into a power of two of pieces of 8 steps at least; long pieces once
+    // more, for a second workgroup on the CU (1024 tokens x 12544 x 1024: 56 -> 42 us with the sums of the two halves;
+    // 1024 x 1024 x 1024 would take 14 instead of 8)
+    long long splits = 1;
+    while (steps / (2 * splits) >= (tiles * splits < kCUs ? 8 : 32) && tiles * splits < 2 * kCUs) splits *= 2;
     p.steps_per = (int)ceil_div(steps, splits);
     p.splits = (int)ceil_div(steps, p.steps_per);
     if (p.splits > 1) p.part_bytes = round_up((size_t)p.splits * tokens * g->channels * sizeof(int), 256);
@@ -710,29 +900,26 @@ int run_prepare(Int8Args &a, int dtype, bool repack, hipStream_t s)
     return check_launch("int8 prepare");
 }
 
-template <int DT, bool NCHW, bool PART, int MI, int NWN, int NS> int launch_tiles(const Int8Args &a, int splits, hipStream_t s)
+template <int DT, bool NCHW, bool PART, int MI, int NWN, int NS> int launch_tiles(const Int8Args &a, hipStream_t s)
 {
     constexpr int BR = 2 * MI * 32, BC = 64 * NWN, kLds = NS * (BR + BC) * 64;
     static std::atomic<uint64_t> done{0};
     if (!raise_lds_limit((const void *)gemm8_kernel<DT, NCHW, PART, MI, NWN, NS>, kLds, done)) return fail(DDCN_ERR_LAUNCH, "int8 product: LDS limit");
     const long long rows = NCHW ? a.tokens : a.channels, cols = NCHW ? a.channels : a.tokens;
-    gemm8_kernel<DT, NCHW, PART, MI, NWN, NS><<<dim3((unsigned)(ceil_div(rows, BR) * ceil_div(cols, BC)), (unsigned)splits), 128 * NWN, kLds, s>>>(a);
+    gemm8_kernel<DT, NCHW, PART, MI, NWN, NS><<<(unsigned)(ceil_div(rows, BR) * ceil_div(cols, BC) * a.splits), 128 * NWN, kLds, s>>>(a);
     return check_launch("int8 product");
 }
 template <int DT, bool NCHW, bool PART> int launch_gemm(const Int8Args &a, const Plan &p, hipStream_t s)
 {
-    if (!p.small) return launch_tiles<DT, NCHW, PART, 2, 2, 2>(a, p.splits, s);
-    return launch_tiles<DT, NCHW, PART, 1, 1, 4>(a, p.splits, s);
+    if (!p.small) return launch_tiles<DT, NCHW, PART, 2, 2, 2>(a, s);
+    return launch_tiles<DT, NCHW, PART, 1, 1, 4>(a, s);
 }
 template <int DT, bool NCHW> int launch_product(const Int8Args &a, const Plan &p, hipStream_t s)
 {
-    if (p.gemv) {
-        const unsigned grid = (unsigned)ceil_div(a.channels, 4);
-        if (a.tokens == 1) gemv8_kernel<DT, NCHW, 1><<<grid, 256, 0, s>>>(a);
-        else if (a.tokens <= 4) gemv8_kernel<DT, NCHW, 4><<<grid, 256, 0, s>>>(a);
-        else gemv8_kernel<DT, NCHW, 16><<<grid, 256, 0, s>>>(a);
-        return check_launch("int8 product");
-    }
+    const unsigned waves = (unsigned)ceil_div(a.channels, 4);
+    if (p.how == kGemv) gemv8_kernel<DT, DDCN_F32, NCHW, 16, false><<<waves, 256, 0, s>>>(a);
+    if (p.how == kDirect) direct8_kernel<DT, NCHW><<<(unsigned)(ceil_div(a.tokens, 64) * ceil_div(a.channels, 32)), 512, 0, s>>>(a);
+    if (p.how != kTiles) return check_launch("int8 product");
     if (p.splits == 1) return launch_gemm<DT, NCHW, false>(a, p, s);
     const int rc = launch_gemm<DDCN_F32, NCHW, true>(a, p, s);
     if (rc != DDCN_OK) return rc;
@@ -744,6 +931,26 @@ template <bool NCHW> int run_product(const Int8Args &a, const Plan &p, int dtype
     if (dtype == DDCN_F32) return launch_product<DDCN_F32, NCHW>(a, p, s);
     if (dtype == DDCN_BF16) return launch_product<DDCN_BF16, NCHW>(a, p, s);
     return launch_product<DDCN_F16, NCHW>(a, p, s);
+}
+
+template <int DT, int IN, bool NCHW> void launch_fused(const Int8Args &a, hipStream_t s)
+{
+    const unsigned waves = (unsigned)ceil_div(a.channels, 4);
+    if (a.tokens == 1) gemv8_kernel<DT, IN, NCHW, 1, true><<<waves, 256, a.chunks * 16, s>>>(a);
+    else gemv8_kernel<DT, IN, NCHW, kFusedTokens, true><<<waves, 256, a.chunks * 16 * kFusedTokens, s>>>(a);
+}
+template <int DT, bool NCHW> void launch_fused_of(const Int8Args &a, int in, hipStream_t s)
+{
+    if (in == DDCN_F32) launch_fused<DT, DDCN_F32, NCHW>(a, s);
+    else if (in == DDCN_BF16) launch_fused<DT, DDCN_BF16, NCHW>(a, s);
+    else launch_fused<DT, DDCN_F16, NCHW>(a, s);
+}
+template <bool NCHW> int run_fused(const Int8Args &a, int in, int out, hipStream_t s)
+{
+    if (out == DDCN_F32) launch_fused_of<DDCN_F32, NCHW>(a, in, s);
+    else if (out == DDCN_BF16) launch_fused_of<DDCN_BF16, NCHW>(a, in, s);
+    else launch_fused_of<DDCN_F16, NCHW>(a, in, s);
+    return check_launch("int8 product");
 }
 
 Int8Args args_of(const ddcn_int8_geom *g)
@@ -768,7 +975,7 @@ size_t ddcn_int8_workspace_bytes(const ddcn_int8_geom *g)
 {
     if (check(g, true) != DDCN_OK || !tokens_of(g)) return 0;
     const long long tokens = tokens_of(g);
-    return plan_of(g, tokens < kPassTokens ? tokens : kPassTokens).bytes();
+    return plan_of(g, tokens < kPassTokens ? tokens : kPassTokens, true).bytes();
 }
 
 int ddcn_int8_product(const void *x, const void *weight, const float *weight_scale, const float *bias, void *y,
@@ -777,9 +984,9 @@ int ddcn_int8_product(const void *x, const void *weight, const float *weight_sca
     int rc = check(g, true);
     if (rc != DDCN_OK) return rc;
     if (!tokens_of(g)) return DDCN_OK;
-    if (!x || !weight || !weight_scale || !y || !workspace) return fail(DDCN_ERR_BAD_ARG, "a pointer is NULL");
-    if ((uintptr_t)workspace & 255) return fail(DDCN_ERR_BAD_ARG, "workspace must be 256-byte aligned");
     const size_t need = ddcn_int8_workspace_bytes(g);
+    if (!x || !weight || !weight_scale || !y || (need && !workspace)) return fail(DDCN_ERR_BAD_ARG, "a pointer is NULL");
+    if ((uintptr_t)workspace & 255) return fail(DDCN_ERR_BAD_ARG, "workspace must be 256-byte aligned");
     if (workspace_bytes < need) return fail(DDCN_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
     Int8Args a = args_of(g);
     a.x = x;
@@ -790,16 +997,22 @@ int ddcn_int8_product(const void *x, const void *weight, const float *weight_sca
     const long long total = tokens_of(g);
     for (a.t0 = 0; a.t0 < total; a.t0 += kPassTokens) {    // (later passes fit the first one's workspace)
         a.tokens = (int)(total - a.t0 < kPassTokens ? total - a.t0 : kPassTokens);
-        const Plan p = plan_of(g, a.tokens);
+        const Plan p = plan_of(g, a.tokens, (((uintptr_t)weight | (uintptr_t)g->ldw) & 15) == 0);
+        if (p.how == kFused) {
+            rc = g->nchw ? run_fused<true>(a, g->dtype, g->out_dtype, (hipStream_t)stream) : run_fused<false>(a, g->dtype, g->out_dtype, (hipStream_t)stream);
+            if (rc != DDCN_OK) return rc;
+            continue;
+        }
         char *ws = (char *)workspace;
         a.ldq = a.tokens;
         a.q = (u32x4 *)ws;
         a.scale = (float *)(ws += p.q_bytes);
         a.wp = (u32x4 *)(ws += p.scale_bytes);
         a.part = (int *)(ws += p.w_bytes);
+        a.splits = p.splits;
         a.steps_per = p.steps_per;
         if ((size_t)(ws - (char *)workspace) + p.part_bytes > workspace_bytes) return fail(DDCN_ERR_WORKSPACE, "workspace too small for the last pass");
-        rc = run_prepare(a, g->dtype, !p.gemv, (hipStream_t)stream);
+        rc = run_prepare(a, g->dtype, p.how == kTiles, (hipStream_t)stream);
         if (rc != DDCN_OK) return rc;
         rc = g->nchw ? run_product<true>(a, p, g->out_dtype, (hipStream_t)stream) : run_product<false>(a, p, g->out_dtype, (hipStream_t)stream);
         if (rc != DDCN_OK) return rc;

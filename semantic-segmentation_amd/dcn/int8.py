@@ -13,65 +13,79 @@ import torch.nn as nn
 from . import _lib
 
 
-def _check_input(name, t):
+_F32 = torch.float32
+_INT8 = torch.int8
+
+
+def _element_type(name, t):
+    """ddcn element type of a floating-point tensor on the GPU that needs no gradient."""
     if not t.is_cuda:
         raise NotImplementedError
-    if t.dtype not in _lib.ELEMENT_TYPES:
+    code = _lib.ELEMENT_TYPES.get(t.dtype)
+    if code is None:
         raise RuntimeError("ddcn: %s of %s is not supported (float32, float16, bfloat16)" % (name, t.dtype))
-    if torch.is_grad_enabled() and t.requires_grad:
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("ddcn: the 8-bit layers have no backward pass: call them under torch.no_grad(), or detach %s"
                            % name)
+    return code
 
 
-def _check_weight(x, weight_q, weight_scale, bias, k):
-    """-> (channels, float32 bias)"""
-    for name, t in (("weight_q", weight_q), ("weight_scale", weight_scale), ("bias", bias)):
-        if t is not None and not t.is_cuda:
+def _check_same_device(name, t, dev, x):
+    if t.get_device() != dev:
+        if not t.is_cuda:
             raise NotImplementedError
-        if t is not None and t.device != x.device:
-            raise RuntimeError("ddcn: %s is on %s but the input is on %s" % (name, t.device, x.device))
-    if weight_q.dtype != torch.int8 or weight_q.dim() != 2 or weight_q.shape[1] != k:
-        raise RuntimeError("ddcn: weight_q has to be int8 [channels, %d], got %s %s" % (k, weight_q.dtype, tuple(weight_q.shape)))
-    n = weight_q.shape[0]
-    if weight_scale.dtype != torch.float32 or weight_scale.shape != (n,):
+        raise RuntimeError("ddcn: %s is on %s but the input is on %s" % (name, t.device, x.device))
+
+
+def _check_weight(x, dev, weight_q, weight_scale, bias, k):
+    """-> (channels, weights with contiguous values in a row, the rows' stride in bytes, scales, float32 bias)"""
+    _check_same_device("weight_q", weight_q, dev, x)
+    _check_same_device("weight_scale", weight_scale, dev, x)
+    shape = weight_q.shape
+    if weight_q.dtype is not _INT8 or len(shape) != 2 or shape[1] != k:
+        raise RuntimeError("ddcn: weight_q has to be int8 [channels, %d], got %s %s" % (k, weight_q.dtype, tuple(shape)))
+    n = shape[0]
+    if weight_scale.dtype is not _F32 or weight_scale.shape != (n,):
         raise RuntimeError("ddcn: weight_scale has to be float32 [%d], got %s %s" % (n, weight_scale.dtype, tuple(weight_scale.shape)))
     if bias is not None:
+        _check_same_device("bias", bias, dev, x)
         if bias.dtype not in _lib.ELEMENT_TYPES or bias.shape != (n,):
             raise RuntimeError("ddcn: bias has to be floating point [%d], got %s %s" % (n, bias.dtype, tuple(bias.shape)))
-        _check_input("bias", bias)
-        bias = bias.detach().float().contiguous()
-    return n, bias
+        _element_type("bias", bias)
+        if bias.dtype is not _F32 or not bias.is_contiguous():
+            bias = bias.detach().float().contiguous()
+    ldw = k
+    if not weight_q.is_contiguous():
+        ldw, one = weight_q.stride()
+        if one != 1 and k > 1 or n > 1 and ldw < k:
+            weight_q, ldw = weight_q.contiguous(), k
+        elif n == 1:
+            ldw = k
+    return n, weight_q, ldw, weight_scale if weight_scale.is_contiguous() else weight_scale.contiguous(), bias
 
 
-def _weight_rows(weight_q):
-    """The weights with contiguous values in a row, and the rows' stride in bytes."""
-    if weight_q.stride(1) != 1 and weight_q.shape[1] > 1 or weight_q.shape[0] > 1 and weight_q.stride(0) < weight_q.shape[1]:
-        weight_q = weight_q.contiguous()
-    return weight_q, max(weight_q.stride(0), weight_q.shape[1])
-
-
-def _product(x, y, weight_q, weight_scale, bias, geom):
+def _product(x, y, dev, weight_q, weight_scale, bias, geom):
     L = _lib.lib()
+    ptr = _lib.ptr
     nbytes = L.ddcn_int8_workspace_bytes(geom)
-    dev = x.get_device()
     with _lib.on_device(dev):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _lib.check(L.ddcn_int8_product(_lib.ptr(x), _lib.ptr(weight_q), _lib.ptr(weight_scale), _lib.ptr(bias),
-                                       _lib.ptr(y), _lib.ptr(ws), nbytes, geom, _lib.stream_of(dev)))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        _lib.check(L.ddcn_int8_product(ptr(x), ptr(weight_q), ptr(weight_scale), ptr(bias), ptr(y), ptr(ws), nbytes,
+                                       geom, _lib.stream_of(dev)))
     return y
 
 
-def _out_dtype(x, out_dtype):
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _lib.ELEMENT_TYPES:
-        raise RuntimeError("ddcn: output of %s is not supported (float32, float16, bfloat16)" % out_dtype)
-    return out_dtype
+def _out_type(dtype):
+    code = _lib.ELEMENT_TYPES.get(dtype)
+    if code is None:
+        raise RuntimeError("ddcn: output of %s is not supported (float32, float16, bfloat16)" % dtype)
+    return code
 
 
 def quantize_int8(x):
     """(q, scale) of the rows of x [rows, k]: int8 [rows, k] and float32 [rows], x ~ q * scale[:, None].  This is the
     rounding of the tokens of `int8_linear`, and the one to lay a weight [channels, k] out with."""
-    _check_input("x", x)
+    code = _element_type("x", x)
     if x.dim() != 2:
         raise RuntimeError("ddcn: 2D tensor expected but got: %d" % x.dim())
     rows, k = x.shape
@@ -79,7 +93,7 @@ def quantize_int8(x):
         x = x.contiguous()
     q = torch.empty((rows, k), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    g = _lib.Int8Geom(1, rows, 1, k, 1, 0, _lib.ELEMENT_TYPES[x.dtype], 0, 0, 0, x.stride(0), 0, 1, k)
+    g = _lib.Int8Geom(1, rows, 1, k, 1, 0, code, 0, 0, 0, x.stride(0), 0, 1, k)
     dev = x.get_device()
     with _lib.on_device(dev):
         _lib.check(_lib.lib().ddcn_int8_quantize(_lib.ptr(x), _lib.ptr(q), k, _lib.ptr(scale), g,
@@ -90,46 +104,48 @@ def quantize_int8(x):
 def int8_linear(input, weight_q, weight_scale, bias=None, relu=False, out_dtype=None):
     """input [..., k] (float32, float16 or bfloat16), weight_q int8 [channels, k], weight_scale float32 [channels],
     bias [channels] -> [..., channels] in `out_dtype` (the input's).  Rows of input may be strided."""
-    _check_input("input", input)
-    if input.dim() < 1:
+    code = _element_type("input", input)
+    shape = input.shape
+    if not shape:
         raise RuntimeError("ddcn: input has no dimension")
-    k = input.shape[-1]
-    n, bias = _check_weight(input, weight_q, weight_scale, bias, k)
-    dtype = _out_dtype(input, out_dtype)
-    x = input.detach().reshape(-1, k) if k else input
-    y = torch.empty(tuple(input.shape[:-1]) + (n,), dtype=dtype, device=input.device)
+    k, dev = shape[-1], input.get_device()
+    n, weight_q, ldw, weight_scale, bias = _check_weight(input, dev, weight_q, weight_scale, bias, k)
+    dtype = input.dtype if out_dtype is None else out_dtype
+    out = _out_type(dtype)
+    y = torch.empty(shape[:-1] + (n,), dtype=dtype, device=input.device)
     if not y.numel():
         return y
-    weight_q, ldw = _weight_rows(weight_q)
-    g = _lib.Int8Geom(1, x.shape[0], 1, k, n, 0, _lib.ELEMENT_TYPES[x.dtype], _lib.ELEMENT_TYPES[dtype], int(relu), 0,
-                      x.stride(0), 0, 1 if k == 1 else x.stride(1), ldw)
-    return _product(x, y, weight_q, weight_scale.contiguous(), bias, g)
+    x = input
+    if len(shape) != 2:
+        x = input.detach().reshape(-1, k)
+    rows, step = x.stride()
+    g = _lib.Int8Geom(1, x.shape[0], 1, k, n, 0, code, out, int(relu), 0, rows, 0, 1 if k == 1 else step, ldw)
+    return _product(x, y, dev, weight_q, weight_scale, bias, g)
 
 
 def int8_conv1x1(input, weight_q, weight_scale, bias=None, stride=1, relu=False, out_dtype=None):
     """1x1 convolution without padding: input [n, c, h, w] (any strides), weight_q int8 [channels, c] ->
     [n, channels, ceil(h / stride), ceil(w / stride)], in channels-last memory where the input is."""
-    _check_input("input", input)
+    code = _element_type("input", input)
     if input.dim() != 4:
         raise RuntimeError("4D input tensor expected but got: %d" % input.dim())
     if int(stride) != stride or stride < 1:
         raise RuntimeError("stride should be greater than zero, but got %r" % (stride,))
     stride = int(stride)
     images, c, h, w = input.shape
-    n, bias = _check_weight(input, weight_q, weight_scale, bias, c)
-    dtype = _out_dtype(input, out_dtype)
+    dev = input.get_device()
+    n, weight_q, ldw, weight_scale, bias = _check_weight(input, dev, weight_q, weight_scale, bias, c)
+    dtype = input.dtype if out_dtype is None else out_dtype
+    out = _out_type(dtype)
     ho, wo = -(-h // stride), -(-w // stride)
-    last = c > 1 and input.stride(1) == 1
+    si, sk, sh, sw = input.stride()
+    last = c > 1 and sk == 1
     y = torch.empty((images, n, ho, wo), dtype=dtype, device=input.device,
                     memory_format=torch.channels_last if last else torch.contiguous_format)
     if not y.numel():
         return y
-    x = input.detach()
-    si, sk, sh, sw = x.stride()
-    weight_q, ldw = _weight_rows(weight_q)
-    g = _lib.Int8Geom(images, ho, wo, c, n, 0 if last else 1, _lib.ELEMENT_TYPES[x.dtype], _lib.ELEMENT_TYPES[dtype],
-                      int(relu), si, sh * stride, sw * stride, sk, ldw)
-    return _product(x, y, weight_q, weight_scale.contiguous(), bias, g)
+    g = _lib.Int8Geom(images, ho, wo, c, n, 0 if last else 1, code, out, int(relu), si, sh * stride, sw * stride, sk, ldw)
+    return _product(input, y, dev, weight_q, weight_scale, bias, g)
 
 
 class _Int8Layer(nn.Module):

@@ -41,7 +41,8 @@ def test_quantize_refuses_bad_arguments():
 
 def test_workspace_holds_codes_and_scales():
     L = _lib.lib()
-    for rows, k in ((1, 1), (10, 100), (1000, 129), (3, 128)):
+    assert L.ddcn_int8_workspace_bytes(_geom(rows=3)) == 0           # one kernel rounds and multiplies
+    for rows, k in ((10, 1), (10, 100), (1000, 129), (3, 131072)):
         least = rows * k + 4 * rows
         got = L.ddcn_int8_workspace_bytes(_geom(rows=rows, k=k, sh=k, ldw=k))
         assert least <= got and got % 256 == 0
