@@ -364,6 +364,8 @@ def inference_workload(args, world, rank, dev):
                               stage_with_dcn=(True, True, True, True), norm_eval=True)
     model = callers.DANet(backbone, callers.DANetHead(2048, 19), None, dcn_offset_init=args.offset_init)
     model = model.to(dev).bfloat16().eval()
+    if args.int8:
+        model = callers.int8_inference(model)
     n = 1 if args.batch == 2 else args.batch
     g = torch.Generator().manual_seed(1234 + rank)
     img = torch.randn(n, 3, 1024, 2048, generator=g).to(dev).bfloat16()
@@ -407,7 +409,7 @@ def inference_workload(args, world, rank, dev):
             "metric": "inference images/sec", "value": round(n * world * args.steps / dt, 3), "unit": "images/s",
             "n_gpus": dist.get_world_size() if world > 1 else 1, "steps": args.steps, "warmup": args.warmup,
             "ms_per_step": round(dt / args.steps * 1e3, 3), "higher_is_better": True, "scaling": "weak",
-            "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
+            "vs_baseline": None, "dtype": "bf16, 1x1 convolutions int8" if args.int8 else "bf16", "data": "synthetic",
             "config": {"workload": "BASELINE configs[4]: ResNet101 with modulated DDCN (dg=4) in all %d bottlenecks + "
                                    "DANet head, 1024x2048 inference, %d image/GPU, random init" % (n_dcn, n),
                        "images_per_gpu": n, "parallelism": "replicas%d" % world, "dcn_offset_init": args.offset_init,
@@ -479,6 +481,7 @@ def main():
                          "(per-layer statistics exchanged over RCCL); default is plain BN per rank")
     ap.add_argument("--sync-allreduce", action="store_true",
                     help="model workloads, N > 1: all-reduce after backward (the reference's order) instead of under it")
+    ap.add_argument("--int8", action="store_true", help="cfg5: 1x1 convolutions in 8-bit integers (an extra figure)")
     ap.add_argument("--no-graph", action="store_true", help="cfg5: launch eagerly instead of replaying a HIP graph")
     ap.add_argument("--backend", choices=("nccl", "gloo"), default="nccl",
                     help="N > 1: 'nccl' = RCCL over xGMI, one GPU per rank (the measured configuration); 'gloo' = a "

@@ -10,9 +10,10 @@ the reference's code implies instead.
 from .resnet import Bottleneck, ResNet, make_res_layer
 from .pointnet import PointNet
 from .danet import CAM_Module, DANet, DANetHead, PAM_Module
+from .int8 import int8_inference
 from .optim import AdamW, adamw_arena, adamw_moments, adamw_step, grad_norm
 from .train import OverlappedGradReducer, build_optimizer, poly_lr, train_step
 
 __all__ = ["Bottleneck", "ResNet", "make_res_layer", "PointNet", "CAM_Module", "DANet", "DANetHead", "PAM_Module",
            "OverlappedGradReducer", "build_optimizer", "poly_lr", "train_step",
-           "AdamW", "adamw_arena", "adamw_moments", "adamw_step", "grad_norm"]
+           "AdamW", "adamw_arena", "adamw_moments", "adamw_step", "grad_norm", "int8_inference"]

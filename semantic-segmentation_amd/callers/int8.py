@@ -1,0 +1,73 @@
+"""Conversion of a trained model for inference in 8 bits: its 1x1 convolutions (with the batch norm behind them) and fully
+connected layers become `Int8Conv1x1` / `Int8Linear`.  Not in the reference; the deformable convolutions, 3x3 convolutions
+and the attention products stay as they are (16-bit under .bfloat16() / .half())."""
+import torch.nn as nn
+from torch.nn.modules.batchnorm import BatchNorm2d
+
+from ..dcn import Int8Conv1x1, Int8Linear
+from ..dcn.deform_conv import _DcnConvBase
+from .resnet import Bottleneck
+
+
+def _pointwise(m, min_channels):
+    return (type(m) is nn.Conv2d and tuple(m.kernel_size) == (1, 1) and m.groups == 1 and m.stride[0] == m.stride[1]
+            and m.padding in ((0, 0), "valid") and m.in_channels >= min_channels)
+
+
+def _norm(m):
+    return type(m) is BatchNorm2d and m.running_mean is not None
+
+
+def _convert_sequence(seq, min_channels):
+    """Conv2d (BatchNorm2d) (ReLU) and Linear (ReLU) runs of a Sequential: one layer, the others become Identity."""
+    names = list(seq._modules)
+    for i, name in enumerate(names):
+        m = seq._modules[name]
+        rest = [seq._modules[n] for n in names[i + 1:i + 3]] + [None, None]
+        if _pointwise(m, min_channels):
+            norm = rest[0] if _norm(rest[0]) else None
+            follows = 1 if norm is None else 2
+            relu = type(rest[follows - 1]) is nn.ReLU
+            seq._modules[name] = Int8Conv1x1.from_float(m, norm, relu)
+        elif type(m) is nn.Linear and m.in_features >= min_channels:
+            follows, relu = 1, type(rest[0]) is nn.ReLU
+            seq._modules[name] = Int8Linear.from_float(m, relu)
+        else:
+            continue
+        for n in names[i + 1:i + follows + (1 if relu else 0)]:
+            seq._modules[n] = nn.Identity()
+
+
+def _convert(module, min_channels):
+    if isinstance(module, _DcnConvBase):         # their inner convolutions place samples: left exact
+        return
+    if isinstance(module, Bottleneck):
+        if _pointwise(module.conv1, min_channels) and _norm(module.bn1):
+            module.conv1, module.bn1, module.relu1 = Int8Conv1x1.from_float(module.conv1, module.bn1, True), nn.Identity(), False
+        if _pointwise(module.conv3, min_channels) and _norm(module.bn3):
+            module.conv3, module.bn3 = Int8Conv1x1.from_float(module.conv3, module.bn3), nn.Identity()
+    elif isinstance(module, nn.Sequential):
+        _convert_sequence(module, min_channels)
+    else:
+        for name, m in module._modules.items():
+            if _pointwise(m, min_channels):
+                module._modules[name] = Int8Conv1x1.from_float(m)
+            elif type(m) is nn.Linear and m.in_features >= min_channels:
+                module._modules[name] = Int8Linear.from_float(m)
+    for m in module._modules.values():
+        if m is not None:
+            _convert(m, min_channels)
+
+
+def int8_inference(model, min_channels=16):
+    """Converts `model` in place and returns it.  It has to be on the GPU and in eval mode: running statistics are folded
+    into the weights, and the converted layers have no backward pass.  Layers with fewer than `min_channels` inputs are
+    left (a token's rounding costs as much as their product).  State dicts of the model change with its layers."""
+    if model.training:
+        raise RuntimeError("ddcn: int8_inference folds running statistics: call model.eval() first")
+    if _pointwise(model, min_channels):
+        return Int8Conv1x1.from_float(model)
+    if type(model) is nn.Linear:
+        return Int8Linear.from_float(model)
+    _convert(model, min_channels)
+    return model

@@ -17,6 +17,7 @@ _DCN_OPS = {"deform": DeformConvPack, "modulated": ModulatedDeformConvPack, "dep
 class Bottleneck(nn.Module):
     """R:85-262, style 'pytorch' (the stride sits on the 3x3 conv)."""
     expansion = 4
+    relu1 = True            # False where conv1 applies the first ReLU itself (callers/int8.py)
 
     def __init__(self, inplanes, planes, stride=1, dilation=1, downsample=None, dcn=None):
         super().__init__()
@@ -53,7 +54,8 @@ class Bottleneck(nn.Module):
         depth = None
         if self.takes_depth:
             x, depth = x
-        out = self.relu(self.bn1(self.conv1(x)))
+        out = self.bn1(self.conv1(x))
+        out = self.relu(out) if self.relu1 else out
         out = self.conv2(out, depth) if self.takes_depth else self.conv2(out)
         out = self.relu(self.bn2(out))
         out = self.bn3(self.conv3(out))

@@ -10,14 +10,22 @@ import torch.distributed as dist
 
 from .. import dist_utils
 from ..dist_utils import allreduce_grads
+from .optim import AdamW
 
 # configs/*/danet_*_depthdeform.py: backbone x1, head x10, depth backbone x10
 PARAMGROUPS = (dict(params="backbone", lr_mult=1), dict(params="head", lr_mult=10),
                dict(params="backbone_depth", lr_mult=10))
 
 
-def build_optimizer(model, lr=0.00025, momentum=0.9, weight_decay=0.0001, paramgroup_options=PARAMGROUPS):
-    """SGD with one parameter group per named sub-module, lr = base * lr_mult (train.py:96-104)."""
+def build_optimizer(model, lr=0.00025, momentum=0.9, weight_decay=0.0001, paramgroup_options=PARAMGROUPS, optimizer="sgd",
+                    max_norm=None, **kwargs):
+    """One parameter group per named sub-module, lr = base * lr_mult (train.py:96-104).  `optimizer`: "sgd" as in the
+    reference, or "adamw" / "adamw8bit" (callers/optim.py, moments in float32 / in 8-bit codes; `max_norm` clips the global
+    gradient norm, `kwargs` go to the optimizer; no momentum)."""
+    if optimizer not in ("sgd", "adamw", "adamw8bit"):
+        raise ValueError("optimizer %r: sgd, adamw or adamw8bit" % (optimizer,))
+    if optimizer == "sgd" and max_norm is not None:
+        raise ValueError("max_norm: with adamw and adamw8bit only")
     model = getattr(model, "module", model)
     groups = []
     for opt in paramgroup_options:
@@ -25,7 +33,9 @@ def build_optimizer(model, lr=0.00025, momentum=0.9, weight_decay=0.0001, paramg
         if sub is None:
             continue
         groups.append(dict(params=list(sub.parameters()), lr=lr * opt["lr_mult"], initial_lr=lr * opt["lr_mult"]))
-    return torch.optim.SGD(groups, lr=lr, momentum=momentum, weight_decay=weight_decay)
+    if optimizer == "sgd":
+        return torch.optim.SGD(groups, lr=lr, momentum=momentum, weight_decay=weight_decay, **kwargs)
+    return AdamW(groups, lr=lr, weight_decay=weight_decay, bits=8 if optimizer == "adamw8bit" else 32, max_norm=max_norm, **kwargs)
 
 
 def poly_lr(optimizer, it, max_iters, power=0.9, min_lr=0.0):
@@ -37,7 +47,7 @@ def poly_lr(optimizer, it, max_iters, power=0.9, min_lr=0.0):
 
 def train_step(model, optimizer, batch, it=0, max_iters=1, ignore_index=255, bucket_size_mb=32, reducer=None,
                amp_dtype=None):
-    """One iteration: poly lr, forward, loss, backward, gradient all-reduce when distributed, SGD update.
+    """One iteration: poly lr, forward, loss, backward, gradient all-reduce when distributed, optimizer update.
     `batch` = dict(img, HHA, gt_label) already on the device.  With `reducer` (an OverlappedGradReducer built on
     the model) the all-reduce runs under backward; otherwise after it, as in the reference.  Returns the loss.
     `amp_dtype` (torch.bfloat16): forward and loss under torch.autocast -- fp32 parameters and optimizer, 16-bit

@@ -50,6 +50,9 @@ def parse_args(argv=None):
                              "stored in the checkpoint; default: --iters of the first run")
     parser.add_argument("--crop", type=int, nargs=2, default=None, metavar=("H", "W"), help="override the crop size")
     parser.add_argument("--imgs_per_gpu", type=int, default=None)
+    parser.add_argument("--optimizer", choices=("sgd", "adamw", "adamw8bit"), default="sgd",
+                        help="sgd as in the reference; adamw with moments in float32 or in 8-bit codes")
+    parser.add_argument("--max_norm", type=float, default=None, help="clip the global gradient norm (adamw, adamw8bit)")
     parser.add_argument("--log_interval", type=int, default=10)
     args = parser.parse_args(argv)
     if "LOCAL_RANK" not in os.environ:
@@ -102,7 +105,7 @@ def main(argv=None):
     model = callers.DANet(backbone, callers.DANetHead(2048, cfg["classes"]), callers.PointNet()).to(dev).train()
     if distributed and world > 1 and cfg["norm"] == "SyncBN":
         model = torch.nn.SyncBatchNorm.convert_sync_batchnorm(model)
-    opt = callers.build_optimizer(model, lr=lr)
+    opt = callers.build_optimizer(model, lr=lr, optimizer=args.optimizer, max_norm=args.max_norm)
     start, max_iters = 0, args.max_iters
     if args.resume_from:
         ck = torch.load(args.resume_from, map_location=dev, weights_only=True)
