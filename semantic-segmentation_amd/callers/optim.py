@@ -6,7 +6,6 @@ The moments of a step live in one arena per moment: tensor i starts at the next 
 i - 1 (`adamw_arena` gives the length).  In 8 bits `exp_avg` is int8, `exp_avg_sq` uint8, each with one float32 scale per
 256 elements: 2.03 bytes a parameter instead of 8.  CPU tensors raise NotImplementedError; there is no fallback.
 """
-import copy
 import ctypes
 from array import array
 from operator import attrgetter
@@ -34,10 +33,19 @@ def _one_device(tensors, name):
     return where.pop()
 
 
-def _check_layout(tensors, name):
+def _all_contiguous(tensors):
     # (a sparse tensor raises a RuntimeError of torch's own here)
-    if not all(map(_Tensor.is_contiguous, tensors)):
-        raise RuntimeError("ddcn: %s tensors have to be contiguous" % name)
+    return all(map(_Tensor.is_contiguous, tensors))
+
+
+def _dense(t):
+    """Contiguous, or channels-last."""
+    return t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)) or \
+        (t.dim() == 5 and t.is_contiguous(memory_format=torch.channels_last_3d))
+
+
+def _same_order(a, b):
+    return a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous())
 
 
 def _arena_of(numels):
@@ -59,7 +67,8 @@ def grad_norm(grads):
     if not grads:
         raise RuntimeError("ddcn: grad_norm needs at least one gradient")
     dev = _one_device(grads, "gradients")
-    _check_layout(grads, "gradient")
+    if not _all_contiguous(grads) and not all(map(_dense, grads)):
+        raise RuntimeError("ddcn: gradient tensors have to be contiguous (or channels-last)")
     try:
         dtypes = array("i", map(_lib.ELEMENT_TYPES.__getitem__, map(_dtype_of, grads)))
     except KeyError as e:
@@ -87,9 +96,11 @@ def _check_state(name, t, dtype, numel, device):
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                exp_avg_scale=None, exp_avg_sq_scale=None, seed=0, grad_norm=None, max_norm=None):
-    """One AdamW step over `params` (list of tensors of one type: float32, bfloat16 or float16), in place.
+    """One AdamW step over `params` (list of tensors of one type: float32, bfloat16 or float16), in place.  They are
+    contiguous or channels-last and do not overlap.
 
-    `grads`: as many tensors of the same shapes and type; None leaves a parameter and its moments as they are.
+    `grads`: as many tensors of the same shapes, type and order in memory; None leaves a parameter and its moments as they
+    are.  (Moments lie in the arena in the order of the parameter's memory.)
     `exp_avg`, `exp_avg_sq`: the arenas (`adamw_arena(params)` elements): float32, or int8 and uint8 with
     `exp_avg_scale`, `exp_avg_sq_scale` (float32, one per 256 elements) and `seed`, a whole number that should differ
     from step to step: it drives the unbiased rounding of the codes, and the same seed gives the same codes.
@@ -112,8 +123,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
         raise RuntimeError("ddcn: %s parameters are not supported (float32, float16, bfloat16)" % dtype)
     if set(map(_dtype_of, params)) | set(map(_dtype_of, given)) != {dtype}:
         raise RuntimeError("ddcn: the parameters and gradients of one step must share a dtype (%s)" % dtype)
-    _check_layout(params, "parameter")
-    _check_layout(given, "gradient")
+    if not _all_contiguous(mine) or not _all_contiguous(given):
+        if not all(p.stride() == g.stride() and _dense(p) for p, g in zip(mine, given)):
+            raise RuntimeError("ddcn: parameters have to be contiguous (or channels-last), gradients in the same order")
     numels = array("q", map(_Tensor.numel, params))
     if array("q", map(_Tensor.numel, given)) != (numels if mine is params else array("q", map(_Tensor.numel, mine))):
         raise RuntimeError("ddcn: a gradient has another number of elements than its parameter")
@@ -158,8 +170,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
                                      _lib.ptr(exp_avg_sq), _lib.ptr(exp_avg_scale), _lib.ptr(exp_avg_sq_scale),
                                      _lib.ptr(grad_norm), hyper, _lib.stream_of(dev)))
     # the kernels write behind autograd's back: a backward pass that saved one of these must notice
-    torch.autograd.graph.increment_version(mine + [exp_avg, exp_avg_sq] +
-                                           ([exp_avg_scale, exp_avg_sq_scale] if bits == 8 else []))
+    changed = mine + [exp_avg, exp_avg_sq] + ([exp_avg_scale, exp_avg_sq_scale] if bits == 8 else [])
+    if torch.is_inference_mode_enabled() or exp_avg.is_inference():      # such tensors keep no versions
+        changed = [t for t in changed if not t.is_inference()]
+    torch.autograd.graph.increment_version(changed)
 
 
 def adamw_moments(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
@@ -196,7 +210,7 @@ class _Arena:
 
     @staticmethod
     def key_of(params):
-        return tuple(map(id, params)), tuple(map(_Tensor.numel, params))
+        return tuple(map(id, params)), tuple(map(_Tensor.stride, params)), tuple(map(_Tensor.numel, params))
 
     def views(self, params):
         """For each parameter: its part of the arena, under the names of the state dict."""
@@ -204,8 +218,8 @@ class _Arena:
         for p in params:
             n = p.numel()
             end = start + -(-n // BLOCK) * BLOCK
-            state = dict(exp_avg=self.exp_avg[start:start + n].view(p.shape),
-                         exp_avg_sq=self.exp_avg_sq[start:start + n].view(p.shape))
+            shaped = lambda t: torch.as_strided(t, p.shape, p.stride(), start)                   # noqa: E731, B023
+            state = dict(exp_avg=shaped(self.exp_avg), exp_avg_sq=shaped(self.exp_avg_sq))
             state.update({k: t[start // BLOCK:end // BLOCK] for k, t in self.scales.items()})
             yield state
             start = end
@@ -264,6 +278,8 @@ class AdamW(torch.optim.Optimizer):
             if all(x is None for x in gs):
                 continue
             group, arena, state = self.param_groups[g], self._arena(g, dtype, params), self.state
+            if not _all_contiguous(params) or not _all_contiguous([x for x in gs if x is not None]):
+                gs = [x if x is None or x.stride() == p.stride() else torch.empty_like(p).copy_(x) for p, x in zip(params, gs)]
             steps = [state[p]["step"] + (x is not None) for p, x in zip(params, gs)]
             same = steps[0] if steps.count(steps[0]) == len(steps) else None
             # a seed for every step and arena; step numbers of one arena only grow
@@ -278,34 +294,48 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As torch's, but moments keep their types (torch would cast them to the parameter's) and are copied into the
         arenas.  A state of another number of bits is refused."""
-        saved = state_dict["state"]
-        super().load_state_dict(dict(state_dict, state={}))
-        self._arenas.clear()
-        self.state.clear()
-        order = {}
+        saved, order = state_dict["state"], {}
         for group, old in zip(self.param_groups, state_dict["param_groups"]):
             order.update(zip(group["params"], old["params"]))
+        loaded = {p: saved[i] for p, i in order.items() if i in saved}
+        want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.bits == 8 else set())
+        for p, theirs in loaded.items():
+            if set(theirs) != want or (theirs["exp_avg"].dtype == torch.int8) != (self.bits == 8) or \
+                    theirs["exp_avg"].shape != p.shape:
+                raise ValueError("the state dict holds %s, not the state of AdamW with bits=%d over these parameters"
+                                 % ({k: getattr(t, "dtype", t) for k, t in theirs.items()}, self.bits))
+        super().load_state_dict(dict(state_dict, state={}))
+        self._take(loaded)
+
+    def _take(self, loaded):
+        """Arenas made anew, with the moments of `loaded` (parameter -> state)."""
+        self._arenas.clear()
+        self.state.clear()
         for g in range(len(self.param_groups)):
             for dtype, params in self._sets(g):
-                if not any(order[p] in saved for p in params):
+                if not any(p in loaded for p in params):
                     continue
                 self._arena(g, dtype, params)
                 for p in params:
-                    mine, theirs = self.state[p], saved.get(order[p])
-                    if theirs is None:
-                        continue
-                    if set(theirs) != set(mine):
-                        raise ValueError("the state dict holds %s, this optimizer %s" % (sorted(theirs), sorted(mine)))
-                    for k, t in theirs.items():
+                    for k, t in loaded.get(p, {}).items():
+                        mine = self.state[p]
                         if k == "step":
                             mine[k] = int(t)
-                        elif t.dtype != mine[k].dtype or t.shape != mine[k].shape:
-                            raise ValueError("%s of the state dict is %s %s, not %s %s" % (
-                                k, t.dtype, tuple(t.shape), mine[k].dtype, tuple(mine[k].shape)))
-                        else:
-                            mine[k].copy_(t)
+                            continue
+                        if self.bits == 8 and not _same_order(t, mine[k]):      # codes and their scales go by memory
+                            raise ValueError("8-bit moments of a parameter in another memory format")
+                        mine[k].copy_(t)
 
-    def __deepcopy__(self, memo):
-        new = type(self)(copy.deepcopy(self.param_groups, memo), bits=self.bits, max_norm=self.max_norm, seed=self.seed)
-        new.load_state_dict(self.state_dict())
-        return new
+    def __getstate__(self):          # copy.deepcopy and pickle: torch's own leaves a subclass's attributes out
+        return dict(super().__getstate__(), settings=(self.bits, self.max_norm, self.seed))
+
+    def __setstate__(self, state):
+        state = dict(state)
+        settings = state.pop("settings", None)
+        super().__setstate__(state)
+        if settings is None:         # from load_state_dict, which takes the moments itself
+            return
+        self.bits, self.max_norm, self.seed = settings
+        self._arenas, self.last_grad_norm = {}, None
+        with torch.no_grad():
+            self._take({p: dict(s) for p, s in self.state.items()})

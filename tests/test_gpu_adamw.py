@@ -371,3 +371,97 @@ def test_optimizer_with_parameters_of_several_types():
     with pytest.raises(RuntimeError, match="changed"):
         opt.param_groups[0]["params"].pop()
         opt.step()
+
+
+def test_channels_last_parameters():
+    """The moments follow the parameter's memory; a gradient in another order is refused by the step and reordered by the
+    optimizer; the state dict holds values at their logical places."""
+    g = _rng(40)
+    w = torch.randn(5, 6, 3, 3, generator=g).to(DEV).to(memory_format=torch.channels_last)
+    grad = torch.randn(5, 6, 3, 3, generator=g).to(DEV)
+    with pytest.raises(RuntimeError, match="order"):
+        callers.adamw_step([w], [grad], torch.zeros(512, device=DEV), torch.zeros(512, device=DEV), 1, LR)
+    p = torch.nn.Parameter(w.clone(memory_format=torch.preserve_format))
+    q = torch.nn.Parameter(w.contiguous())
+    opts = [callers.AdamW([x], lr=LR, betas=BETAS, weight_decay=WD, max_norm=0.5) for x in (p, q)]
+    for t in range(2):
+        for x, o in zip((p, q), opts):
+            x.grad = grad.clone()
+            o.step()
+        grad = grad * 0.5
+    assert p.is_contiguous(memory_format=torch.channels_last) and torch.equal(p, q)
+    assert torch.equal(opts[0].state[p]["exp_avg"], opts[1].state[q]["exp_avg"])
+    opts[1].load_state_dict(opts[0].state_dict())
+    for x, o in zip((p, q), opts):
+        x.grad = grad.clone()
+        o.step()
+    assert torch.equal(p, q)
+
+
+def test_8_bit_state_of_another_memory_format_is_refused():
+    w = torch.randn(5, 6, 3, 3, generator=_rng(41)).to(DEV)
+    p = torch.nn.Parameter(w.to(memory_format=torch.channels_last))
+    q = torch.nn.Parameter(w)
+    opts = [callers.AdamW([x], bits=8) for x in (p, q)]
+    for x, o in zip((p, q), opts):
+        x.grad = torch.ones_like(x)
+        o.step()
+    with pytest.raises(ValueError, match="memory format"):
+        opts[1].load_state_dict(opts[0].state_dict())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_of_an_optimizer_go_on_by_themselves(bits):
+    import copy
+    import pickle
+    model = _model(5)
+    opt = callers.AdamW(model.parameters(), lr=1e-2, bits=bits, max_norm=1.0, seed=9)
+
+    def step(m, o, t):
+        g = _rng(200 + t)
+        for p in m.parameters():
+            p.grad = torch.randn(p.shape, generator=g).to(DEV)
+        o.step()
+
+    step(model, opt, 0)
+    other, o2 = copy.deepcopy((model, opt))
+    third, o3 = pickle.loads(pickle.dumps((model, opt)))
+    for t in (1, 2):
+        step(model, opt, t)
+    for m, o in ((other, o2), (third, o3)):
+        assert o.param_groups[0]["params"][0] is next(m.parameters())
+        for t in (1, 2):
+            step(m, o, t)
+        assert all(torch.equal(a, b) for a, b in zip(model.parameters(), m.parameters()))
+
+
+def test_step_under_inference_mode():
+    p, g = torch.ones(300, device=DEV), torch.ones(300, device=DEV)
+    m, v = torch.zeros(512, device=DEV), torch.zeros(512, device=DEV)
+    with torch.inference_mode():
+        callers.adamw_step([p], [g], m, v, 1, LR)
+        callers.adamw_step([torch.ones(300, device=DEV)], [g], torch.zeros(512, device=DEV), torch.zeros(512, device=DEV), 1, LR)
+    assert (p < 1).all()
+
+
+def test_steps_of_two_streams_at_once():
+    """Two sets of tensors on two streams: neither sees the other's kernel arguments, workspaces or norm."""
+    sizes = SIZES["many"]
+    sets = []
+    for k in range(2):
+        params, grads = _inputs(sizes, torch.float32, 50 + k)
+        sets.append((params, grads, *_arena32(sizes, 60 + k)))
+    want = [[t.clone() for t in s[0]] + [s[2].clone(), s[3].clone()] for s in sets]
+    for w, s in zip(want, sets):
+        n = len(sizes)
+        for t in range(5):
+            callers.adamw_step(w[:n], s[1], w[n], w[n + 1], t + 1, LR, grad_norm=callers.grad_norm(s[1]), max_norm=0.1)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for t in range(5):
+        for stream, s in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                callers.adamw_step(s[0], s[1], s[2], s[3], t + 1, LR, grad_norm=callers.grad_norm(s[1]), max_norm=0.1)
+    torch.cuda.synchronize()
+    for w, s in zip(want, sets):
+        assert all(torch.equal(a, b) for a, b in zip(w, s[0] + [s[2], s[3]]))
