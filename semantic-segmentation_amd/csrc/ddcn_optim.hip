@@ -136,9 +136,9 @@ __device__ __forceinline__ void encode(const float (&m)[4], const float (&v)[4],
             far_r = fmaxf(far_r, fabsf(__builtin_amdgcn_fractf(xr) - 0.5f));
         }
         const int q = (int)copysignf(fminf(floorf(xm), 127.f), m[e]);
-        const float k = fmaxf(floorf(xr), v[e] > 0.f ? 1.f : 0.f);     // a code of at least 1 where v > 0
         qm |= (unsigned)(q & 255) << (8 * e);
-        qv |= (unsigned)fminf(k, 255.f) << (8 * e);
+        // at most 255, and at least 1 where v > 0
+        qv = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_amdgcn_fmed3f(floorf(xr), v[e] > 0.f ? 1.f : 0.f, 255.f), e, qv);
     }
 }
 
