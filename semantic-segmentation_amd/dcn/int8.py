@@ -158,12 +158,13 @@ class _Int8Layer(nn.Module):
         self.register_buffer("bias", torch.zeros(channels, dtype=torch.float32) if bias else None)
 
     def _apply(self, fn, recurse=True):
-        # .half() / .bfloat16() move a model to 16-bit activations: scales and bias stay float32
+        # .half() / .bfloat16() move a model to 16-bit activations: scales and bias stay float32, unrounded
+        before = {name: getattr(self, name) for name in ("weight_scale", "bias")}
         super()._apply(fn, recurse)
-        for name in ("weight_scale", "bias"):
-            t = getattr(self, name)
-            if t is not None and t.dtype != torch.float32:
-                setattr(self, name, t.float())
+        for name, t in before.items():
+            now = getattr(self, name)
+            if now is not None and now.dtype != torch.float32:
+                setattr(self, name, t.to(now.device))
         return self
 
     @torch.no_grad()

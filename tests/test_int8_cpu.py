@@ -67,3 +67,15 @@ def test_layers_keep_their_scales_in_float32():
     for conv in (torch.nn.Conv2d(4, 4, 3), torch.nn.Conv2d(4, 4, 1, groups=2), torch.nn.Conv2d(4, 4, 1, padding=1)):
         with pytest.raises(ValueError):
             pkg.Int8Conv1x1.from_float(conv)
+
+
+@pytest.mark.parametrize("cast", ["half", "bfloat16"])
+def test_scales_are_not_rounded_when_a_model_moves_to_16_bits(cast):
+    layer = pkg.Int8Linear(8, 4)
+    layer.weight_scale.copy_(torch.tensor([1.2345678e-6, 3.3e-9, 0.7654321, 100.123]))       # float16 would lose the first two
+    layer.bias.copy_(torch.tensor([1.0000001, 1e-9, 70000.5, -0.1]))
+    want = {k: v.clone() for k, v in layer.state_dict().items()}
+    for model in (layer, torch.nn.Sequential(layer)):
+        getattr(model, cast)()
+        assert all(torch.equal(layer.state_dict()[k], v) and layer.state_dict()[k].dtype == v.dtype for k, v in want.items())
+    assert layer.to("meta", torch.float16).weight_scale.device.type == "meta"
