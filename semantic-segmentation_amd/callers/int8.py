@@ -15,7 +15,7 @@ def _pointwise(m, min_channels):
 
 
 def _norm(m):
-    return type(m) is BatchNorm2d and m.running_mean is not None
+    return type(m) is BatchNorm2d and m.running_mean is not None and not m.training
 
 
 def _convert_sequence(seq, min_channels):

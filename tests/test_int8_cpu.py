@@ -79,3 +79,12 @@ def test_scales_are_not_rounded_when_a_model_moves_to_16_bits(cast):
         getattr(model, cast)()
         assert all(torch.equal(layer.state_dict()[k], v) and layer.state_dict()[k].dtype == v.dtype for k, v in want.items())
     assert layer.to("meta", torch.float16).weight_scale.device.type == "meta"
+
+
+def test_a_norm_that_still_learns_is_not_folded():
+    callers = importlib.import_module("semantic-segmentation_amd.callers")
+    block = callers.Bottleneck(64, 16).eval()
+    block.bn1.train(), block.bn3.train()
+    before = list(block.modules())
+    callers.int8_inference(block)
+    assert list(block.modules()) == before and block.relu1
