@@ -124,7 +124,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
     if set(map(_dtype_of, params)) | set(map(_dtype_of, given)) != {dtype}:
         raise RuntimeError("ddcn: the parameters and gradients of one step must share a dtype (%s)" % dtype)
     if not _all_contiguous(mine) or not _all_contiguous(given):
-        if not all(p.stride() == g.stride() and _dense(p) for p, g in zip(mine, given)):
+        if not all(_same_order(p, g) and _dense(p) for p, g in zip(mine, given)):
             raise RuntimeError("ddcn: parameters have to be contiguous (or channels-last), gradients in the same order")
     numels = array("q", map(_Tensor.numel, params))
     if array("q", map(_Tensor.numel, given)) != (numels if mine is params else array("q", map(_Tensor.numel, mine))):
@@ -155,9 +155,6 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
         steps, step = array("i", step), 1
         if len(steps) != len(params):
             raise RuntimeError("ddcn: %d parameters but %d step numbers" % (len(params), len(steps)))
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("ddcn: adamw_step cannot be captured into a HIP graph: a replay would repeat the step number, "
-                           "the learning rate and the seed of the capture")
     hyper = _lib.AdamwHyper(lr, betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, step,
                             _lib.ELEMENT_TYPES[dtype], bits, int(seed) & 0xFFFFFFFF)
     if mine is params:
@@ -165,6 +162,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
     else:
         gradients = array("Q", [0 if g is None else g.data_ptr() for g in grads])
     with _lib.on_device(dev):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("ddcn: adamw_step cannot be captured into a HIP graph: a replay would repeat the step "
+                               "number, the learning rate and the seed of the capture")
         _lib.check(L.ddcn_adamw_step(len(params), _address(pointers), _address(gradients), _address(numels),
                                      None if steps is None else _address(steps), _lib.ptr(exp_avg),
                                      _lib.ptr(exp_avg_sq), _lib.ptr(exp_avg_scale), _lib.ptr(exp_avg_sq_scale),
@@ -279,7 +279,7 @@ class AdamW(torch.optim.Optimizer):
                 continue
             group, arena, state = self.param_groups[g], self._arena(g, dtype, params), self.state
             if not _all_contiguous(params) or not _all_contiguous([x for x in gs if x is not None]):
-                gs = [x if x is None or x.stride() == p.stride() else torch.empty_like(p).copy_(x) for p, x in zip(params, gs)]
+                gs = [x if x is None or _same_order(x, p) else torch.empty_like(p).copy_(x) for p, x in zip(params, gs)]
             steps = [state[p]["step"] + (x is not None) for p, x in zip(params, gs)]
             same = steps[0] if steps.count(steps[0]) == len(steps) else None
             # a seed for every step and arena; step numbers of one arena only grow

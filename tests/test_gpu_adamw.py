@@ -398,6 +398,28 @@ def test_channels_last_parameters():
     assert torch.equal(p, q)
 
 
+def test_pointwise_weights_in_either_format_beside_channels_last_ones():
+    """A [n, c, 1, 1] tensor has one order in memory whatever strides it names."""
+    g = _rng(43)
+    make = lambda *shape: torch.randn(*shape, generator=g).to(DEV)                               # noqa: E731
+    a, b = make(5, 6, 3, 3).to(memory_format=torch.channels_last), make(7, 5, 1, 1).to(memory_format=torch.channels_last)
+    ga, gb = make(5, 6, 3, 3).to(memory_format=torch.channels_last), make(7, 5, 1, 1)
+    assert b.stride() != gb.stride()
+    want = []
+    for x, y in ((a, ga), (b, gb)):
+        w = x.clone()
+        callers.adamw_step([w], [y], *(torch.zeros(callers.adamw_arena([w]), device=DEV) for _ in range(2)), 1, LR)
+        want.append(w)
+    params = [a.clone(), b.clone()]
+    n = callers.adamw_arena(params)
+    callers.adamw_step(params, [ga, gb], torch.zeros(n, device=DEV), torch.zeros(n, device=DEV), 1, LR)
+    assert all(torch.equal(p, w) for p, w in zip(params, want))
+    again = [torch.nn.Parameter(a.clone()), torch.nn.Parameter(b.clone())]
+    again[0].grad, again[1].grad = ga.clone(), gb.clone()
+    callers.AdamW(again, lr=LR).step()
+    assert all(torch.equal(p, w) for p, w in zip(again, want))
+
+
 def test_8_bit_state_of_another_memory_format_is_refused():
     w = torch.randn(5, 6, 3, 3, generator=_rng(41)).to(DEV)
     p = torch.nn.Parameter(w.to(memory_format=torch.channels_last))
