@@ -16,6 +16,8 @@ namespace {
 constexpr int kBlock = 256;             // elements per pair of scales, and per wave and turn
 constexpr int kWaves = 4;
 
+constexpr long long kMaxGrid = 1LL << 23;   // workgroups of a launch: 256 threads each have to stay below 2^32 in all
+
 constexpr int kMaxTensors = 160;
 struct AdamwArgs {
     // tensor j of the launch covers the arena's blocks block0[j] .. block0[j+1]-1 (relative to `first`); n[j] elements.
@@ -494,7 +496,7 @@ int ddcn_adamw_step(int count, const unsigned long long *params, const unsigned 
         // a tensor of 2^31 elements and more goes in pieces
         for (long long done = 0; done < numels[i]; done += 1LL << 31) {
             const long long n = numels[i] - done < (1LL << 31) ? numels[i] - done : 1LL << 31, blocks = ceil_div(n, kBlock);
-            if (a.count == kMaxTensors || a.blocks + blocks > (1LL << 31)) {
+            if (a.count == kMaxTensors || a.blocks + blocks > kMaxGrid * kWaves) {
                 const int rc = launch();
                 if (rc != DDCN_OK) return rc;
             }
@@ -518,11 +520,14 @@ int ddcn_adamw_moments(const void *exp_avg, const void *exp_avg_sq, const float 
     if (!exp_avg || !exp_avg_sq || !exp_avg_scale || !exp_avg_sq_scale || !m || !v) return fail(DDCN_ERR_BAD_ARG, "a pointer is NULL");
     if (((uintptr_t)m | (uintptr_t)v) & 15 || ((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 3)
         return fail(DDCN_ERR_BAD_ARG, "moments: outputs must be 16-byte, codes 4-byte aligned");
-    const long long grid = ceil_div(numel / 4, 256);
-    if (grid >= (1LL << 31)) return fail(DDCN_ERR_UNSUPPORTED, "%lld elements", numel);
-    adamw_moments_kernel<<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>((const signed char *)exp_avg,
-        (const unsigned char *)exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, m, v, numel / 4);
-    return check_launch("adamw_moments");
+    for (long long at = 0; at < numel; at += kMaxGrid * 1024) {
+        const long long quads = (numel - at < kMaxGrid * 1024 ? numel - at : kMaxGrid * 1024) / 4;
+        adamw_moments_kernel<<<(unsigned)ceil_div(quads, 256), 256, 0, (hipStream_t)stream>>>((const signed char *)exp_avg + at,
+            (const unsigned char *)exp_avg_sq + at, exp_avg_scale + at / kBlock, exp_avg_sq_scale + at / kBlock, m + at, v + at, quads);
+        const int rc = check_launch("adamw_moments");
+        if (rc != DDCN_OK) return rc;
+    }
+    return DDCN_OK;
 }
 
 size_t ddcn_grad_norm_workspace_bytes(int count, const long long *numels)
@@ -539,6 +544,7 @@ int ddcn_grad_norm(int count, const unsigned long long *grads, const long long *
     if ((uintptr_t)workspace & 15) return fail(DDCN_ERR_BAD_ARG, "workspace must be 16-byte aligned");
     for (int i = 0; i < count; ++i) {
         if (numels[i] < 0) return fail(DDCN_ERR_SHAPE, "tensor %d has %lld elements", i, numels[i]);
+        if (numels[i] > kMaxGrid * kNormChunk) return fail(DDCN_ERR_UNSUPPORTED, "tensor %d has %lld elements", i, numels[i]);
         if (dtypes[i] < DDCN_F32 || dtypes[i] > DDCN_F16) return fail(DDCN_ERR_UNSUPPORTED, "dtype %d of tensor %d", dtypes[i], i);
         if (numels[i] && !grads[i]) return fail(DDCN_ERR_BAD_ARG, "tensor %d is NULL", i);
         if (grads[i] & (dtypes[i] == DDCN_F32 ? 3 : 1)) return fail(DDCN_ERR_BAD_ARG, "tensor %d is not aligned to its elements", i);
@@ -551,7 +557,7 @@ int ddcn_grad_norm(int count, const unsigned long long *grads, const long long *
     for (int i = 0; i <= count; ++i) {
         const bool end = i == count;
         const long long mine = end ? 0 : ceil_div(numels[i], kNormChunk);
-        if (a.count && (end || a.count == kMaxNorm || chunks + mine >= (1LL << 31))) {
+        if (a.count && (end || a.count == kMaxNorm || chunks + mine > kMaxGrid)) {
             a.partial = (double *)workspace + done;
             norm_partial_kernel<<<(unsigned)chunks, 256, 0, (hipStream_t)stream>>>(a);
             const int rc = check_launch("grad_norm");
@@ -562,7 +568,6 @@ int ddcn_grad_norm(int count, const unsigned long long *grads, const long long *
         }
         if (end) break;
         if (!mine) continue;
-        if (mine >= (1LL << 31)) return fail(DDCN_ERR_UNSUPPORTED, "tensor %d has %lld elements", i, numels[i]);
         NormTensor &t = a.t[a.count++];
         t.g = (const void *)grads[i];
         t.n = numels[i];

@@ -59,6 +59,8 @@ def test_norm_and_moments_refuse_bad_arguments():
     k5, odd = _a("Q", [4098])
     k6, null = _a("Q", [0])
     assert call(g, n, bad_type) == -5 and call(odd, n, t) == -1 and call(null, n, t) == -1
+    k7, endless = _a("q", [(1 << 36) + 1])
+    assert call(g, endless, t) == -5
     assert L.ddcn_adamw_moments(64, 64, 64, 64, 64, 64, 100, None) == -2
     assert L.ddcn_adamw_moments(64, 64, 64, 64, 64, 72, 256, None) == -1
     assert L.ddcn_adamw_moments(None, 64, 64, 64, 64, 64, 256, None) == -1

@@ -487,3 +487,50 @@ def test_steps_of_two_streams_at_once():
     torch.cuda.synchronize()
     for w, s in zip(want, sets):
         assert all(torch.equal(a, b) for a, b in zip(w, s[0] + [s[2], s[3]]))
+
+
+def _needs_memory(gigabytes):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gigabytes * 1e9:
+        pytest.skip("needs %d GB" % gigabytes)
+
+
+def test_arena_of_more_blocks_than_a_grid_has_room_for():
+    """2^35 elements between two tensors that have a gradient: their offsets pass 32 bits, and one launch over all blocks
+    would have 2^32 threads.  The numbers of the rounding repeat every 2^32 elements, so that the same two tensors alone
+    get the same codes."""
+    _needs_memory(90)
+    (p0, p1), (g0, g1) = _inputs([1000, 700], torch.float32, 50)
+    huge = [x.expand(1 << 31) for x in torch.zeros(16, device=DEV).split(1)]
+    got, want = [p0.clone(), p1.clone()], [p0.clone(), p1.clone()]
+    results = []
+    for params, grads in (([got[0], *huge, got[1]], [g0, *[None] * 16, g1]), (want, [g0, g1])):
+        n = callers.adamw_arena(params)
+        m, v = torch.empty(n, dtype=torch.int8, device=DEV), torch.empty(n, dtype=torch.uint8, device=DEV)
+        sm, sv = torch.zeros(n // 256, device=DEV), torch.zeros(n // 256, device=DEV)
+        for at in (slice(0, 1024), slice(n - 768, n)):
+            m[at] = 0
+            v[at] = 0
+        for t in (1, 2):
+            callers.adamw_step(params, grads, m, v, t, LR, BETAS, EPS, WD, sm, sv, t)
+        results.append([x for t, k in ((m, 1), (v, 1), (sm, 256), (sv, 256)) for x in (t[:1024 // k].clone(), t[(n - 768) // k:].clone())])
+    assert n == 1024 + 768
+    assert all(torch.equal(a, b) for a, b in zip(got + results[0], want + results[1]))
+    assert not torch.equal(got[1], p1)
+
+
+def test_moments_of_more_elements_than_a_grid_has_room_for():
+    _needs_memory(110)
+    n = (1 << 33) + 768
+    m, v = torch.zeros(n, dtype=torch.int8, device=DEV), torch.zeros(n, dtype=torch.uint8, device=DEV)
+    sm, sv = torch.zeros(n // 256, device=DEV), torch.zeros(n // 256, device=DEV)
+    parts = (slice(0, 512), slice((1 << 32) - 256, (1 << 32) + 256), slice((1 << 33) - 256, n))
+    for i, at in enumerate(parts):
+        m[at], v[at], x, y = _arena8([at.stop - at.start], 60 + i)
+        sm[at.start // 256:at.stop // 256], sv[at.start // 256:at.stop // 256] = x, y
+    dm, dv = callers.adamw_moments(m, v, sm, sv)
+    for at in parts:
+        s = slice(at.start // 256, at.stop // 256)
+        a, b = callers.adamw_moments(m[at].clone(), v[at].clone(), sm[s].clone(), sv[s].clone())
+        assert torch.equal(dm[at], a) and torch.equal(dv[at], b) and a.any() and b.any()
+    assert not dm[512:4096].any() and not dv[-(1 << 20) - 1024:-1024].any()
