@@ -19,7 +19,9 @@ namespace {
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 
 constexpr int kMaxK = 131072;          // k * 127 * 128 stays below 2^31
-constexpr long long kPassTokens = 1LL << 24;   // tokens of one pass: offsets within four rows of chunks fit 31 bits
+// Tokens of one pass: offsets within four rows of chunks fit 31 bits, and a workgroup of 256 threads for each of them makes
+// a grid of 2^31 threads (below 2^32)
+constexpr long long kPassTokens = 1LL << 23;
 
 struct Int8Args {
     const void *x;

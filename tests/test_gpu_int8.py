@@ -283,3 +283,17 @@ def test_more_tokens_than_one_pass():
     z = pkg.int8_conv1x1(x.view(images, 2, h, k).permute(0, 3, 1, 2).contiguous(), wq, ws, b).permute(0, 2, 3, 1).reshape(-1, n)
     for at in (slice(0, 500), slice((1 << 24) - 500, (1 << 24) + 500), slice(-500, None)):
         assert torch.equal(z[at], pkg.int8_linear(x[at], wq, ws, b))
+
+
+def test_passes_of_long_tokens_and_a_pass_that_ends_inside_an_image():
+    """Long tokens take a workgroup each: no grid of a pass may reach 2^32 threads.  (All rows of x are one row.)"""
+    row = _make((1, 2304), torch.bfloat16, 6)
+    wq, ws, b = _weights(2, 2304, 7)
+    y = pkg.int8_linear(row.expand((1 << 24) + 5, 2304), wq, ws, b, out_dtype=torch.float32)
+    assert (y == pkg.int8_linear(row, wq, ws, b, out_dtype=torch.float32)).all()
+    images, h, w, k, n = 3, 4099, 683, 8, 3                # 2^23 tokens end inside the third image
+    x = torch.randint(-3, 4, (images, h * w, k), device=DEV, generator=torch.Generator(device=DEV).manual_seed(8)).to(torch.float16)
+    wq, ws, b = _weights(n, k, 9)
+    z = pkg.int8_conv1x1(x.view(images, h, w, k).permute(0, 3, 1, 2).contiguous(), wq, ws, b).permute(0, 2, 3, 1).reshape(-1, n)
+    for at in (slice(0, 500), slice((1 << 23) - 500, (1 << 23) + 500), slice(-500, None)):
+        assert torch.equal(z[at], pkg.int8_linear(x.view(-1, k)[at], wq, ws, b))
