@@ -2,9 +2,9 @@
 // stand in include/ddcn_hip.h.
 //
 //   prepare_*    x (any strides) -> codes and the tokens' scales; workgroups behind those of the tokens repack the weights
-//   gemm8        (more than 512 tokens) codes x weights on v_mfma_i32_16x16x64_i8, operands global -> LDS by DMA through a ring of K steps; exact
-//                int32 sums, scales + bias + ReLU in the epilogue, or int32 partial sums where K is split
-//   direct8      (17 to 512 tokens) both operands straight into the MFMA's registers, weights from the caller's rows
+//   gemm8        (many tokens) codes x weights on v_mfma_i32_16x16x64_i8, operands global -> LDS by DMA through a ring of K
+//                steps; exact int32 sums, scales + bias + ReLU in the epilogue, or int32 partial sums where K is split
+//   direct8      (from 17 tokens on, see plan_of) codes straight into the MFMA's registers, weights from the caller's rows
 //   gemv8        (up to 16) a wave per channel streams its weights once, v_dot4_i32_i8; up to 4 tokens it rounds them too
 //   finish       sums of the partial sums, epilogue
 //
@@ -600,127 +600,153 @@ template <int DT, bool NCHW> __global__ __launch_bounds__(256) void finish_kerne
 }
 
 // ---------------------------------------------------------------- few tokens
-// Up to kDirectTokens (512 x 2048 x 512: 8.2 us, tiles with split K 6.4 + 3.1 and the repacking of the weights; 300 x 12544 x
-// 1024: 22.5, tiles 15.5 + 4.3 + 3; above, tiles win): what counts is to stream the weights once, from the caller's own rows (repacking them moves as many
-// bytes again, twice).  64 tokens x 32 channels per workgroup, K dealt to its eight waves in turns of 128 k (a
-// line of a weight row); both operands go
-// straight into the MFMA's registers (a weight fragment is 16 rows x 64 bytes, a code fragment four runs of 256), two
-// turns ahead, and nothing is shared until the waves' sums meet in LDS.
-template <int DT, bool NCHW> __global__ __launch_bounds__(512) void direct8_kernel(const Int8Args a)
+// What counts is to stream the weights once, from the caller's own rows (repacking them moves as many bytes again, twice).
+// 64 tokens x 16 NW channels per workgroup, and a piece of K where PART; K is dealt to the eight waves in turns of 128 k, a
+// line of a weight row, two turns ahead, and nothing is shared until the waves' sums meet in LDS.  A code fragment is four
+// runs of 256 bytes and goes straight into the MFMA's registers.  A weight fragment is 16 rows x 64 bytes: loaded that way
+// every lane of a quarter wave touches another line, 64 line accesses for 1 KB (43 cycles of the data return path a load
+// over both operands, and 300 x 12544 x 1024 took 15.3 us in place of 11.5).  So eight lanes fetch a whole line of a row,
+// by DMA, into the wave's own LDS; there chunk c of row r lies in place c ^ (r % 8), which spreads eight rows over all banks.
+template <int DT, bool NCHW, bool PART, int NW> __global__ __launch_bounds__(512) void direct8_kernel(const Int8Args a)
 {
-    constexpr bool PAIRS = DT != DDCN_F32;
-    constexpr int NR = NCHW ? 4 : 2, NC = NCHW ? 2 : 4;    // tiles of 16 rows (registers, contiguous in y) and columns (lanes)
-    constexpr int kWaves = 8, kAhead = 2;
-    __shared__ i32x4 sums[kWaves][NR * NC][64];
+    constexpr bool PAIRS = !PART && DT != DDCN_F32;
+    constexpr int NR = NCHW ? 4 : NW, NC = NCHW ? NW : 4;    // tiles of 16 rows (registers, contiguous in y) and columns (lanes)
+    constexpr int kWaves = 8, kTurn = 2 * NW;              // requests of a turn's weights
+    extern __shared__ u32x4 ring[];                        // [wave][2 turns][request][64]; after K the waves' sums
+    i32x4 (*sums)[8][64] = (i32x4 (*)[8][64])ring;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kc = lane >> 4;
     // an XCD takes a range of channels and all tokens: its L2 then reads its part of the weights alone
-    const int across = (a.tokens + 63) / 64, L = xcd_logical(blockIdx.x, gridDim.x);
-    const int t0 = L % across * 64, n0 = L / across * 32;
+    const int across = (a.tokens + 63) / 64, down = (a.channels + NW * 16 - 1) / (NW * 16), L = xcd_logical(blockIdx.x, gridDim.x);
+    const int t0 = L % across * 64, n0 = L / across % down * (NW * 16), split = PART ? L / (across * down) : 0;
     const int rows = NCHW ? a.tokens : a.channels, cols = NCHW ? a.channels : a.tokens;
     const int r0 = NCHW ? t0 : n0, c0 = NCHW ? n0 : t0;
-    // this lane's tokens and weight rows (clamped: what is computed for the others is not stored)
-    const u32x4 *qp[4];
-    const signed char *wp[2];
+    // this lane's tokens and, of each request, its weight row and chunk (clamped: what is computed for the others is not
+    // stored), in bytes from the workgroup's first ones
+    const char *qb = (const char *)(a.q + t0);
+    const signed char *wb = a.w + n0 * a.ldw;
+    const int most = min(NW * 16, a.channels - n0) - 1;    // last row
+    unsigned qo[4], wo[kTurn];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) qp[i] = a.q + min(t0 + (NCHW ? row_of<PAIRS>(i * 16 + r16) : i * 16 + r16), a.tokens - 1) + kc * a.ldq;
+    for (int i = 0; i < 4; ++i) qo[i] = (unsigned)(min(NCHW ? row_of<PAIRS>(i * 16 + r16) : i * 16 + r16, a.tokens - 1 - t0) + kc * (int)a.ldq) * 16u;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) wp[i] = a.w + min(n0 + (NCHW ? i * 16 + r16 : row_of<PAIRS>(i * 16 + r16)), a.channels - 1) * a.ldw + kc * 16;
-    struct Frags {
-        u32x4 q[2][4], w[2][2];
-    };
-    const int full = a.k / 128;                            // turns whose weights need no guard
-    auto load = [&](int s) {
-        Frags f;
+    for (int i = 0; i < kTurn; ++i) wo[i] = (unsigned)(min(i * 8 + lane / 8, most) * (int)a.ldw + ((lane ^ lane / 8) & 7) * 16);
+    u32x4 *mine = ring + wave * (2 * kTurn * 64);
+    int at[NW];                                            // of this lane's row in a turn's image, without its chunk
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) f.w[h][i] = *(const u32x4 *)(wp[i] + s * 128 + h * 64);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f.q[h][i] = qp[i][((long long)s * 8 + h * 4) * a.ldq];
-        return f;
-    };
+    for (int i = 0; i < NW; ++i) at[i] = (NCHW ? i * 16 + r16 : row_of<PAIRS>(i * 16 + r16)) * 8;
+    // turns of this piece of K whose weights need no guard
+    const int begin = PART ? split * a.steps_per : 0, full = PART ? min(begin + a.steps_per, a.k / 128) : a.k / 128;
+    const bool last = !PART || split == a.splits - 1;
     i32x4 acc[NR][NC];
 #pragma unroll
     for (int i = 0; i < NR; ++i)
 #pragma unroll
         for (int j = 0; j < NC; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-    auto mul = [&](const Frags &f) {
+    auto mul = [&](const u32x4 (&w)[NW], const u32x4 (&q)[4]) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) acc[i][j] = NCHW ? mfma8(q[i & 3], w[j & (NW - 1)], acc[i][j]) : mfma8(w[i & (NW - 1)], q[j & 3], acc[i][j]);
+    };
+    u32x4 q[2][2][4];
+    auto request = [&](int s, int d) {
+        dma<kTurn, 1024>((const u32x4 *)(wb + s * 128), (unsigned)(most * (int)a.ldw + a.k - s * 128), (char *)(mine + d * (kTurn * 64)), wo);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < NR; ++i)
-#pragma unroll
-                for (int j = 0; j < NC; ++j) acc[i][j] = NCHW ? mfma8(f.q[h][i], f.w[h][j & 1], acc[i][j]) : mfma8(f.w[h][i & 1], f.q[h][j], acc[i][j]);
+            for (int i = 0; i < 4; ++i) q[d][h][i] = *(const u32x4 *)(qb + ((long long)s * 8 + h * 4) * a.ldq * 16 + qo[i]);
     };
-    Frags f[kAhead];
-    int s = wave;
-    // while the next kAhead turns exist, every turn loads one: the number of loads in flight is known, and a turn waits for
-    // its own alone
-    if (s + (2 * kAhead - 1) * kWaves < full) {
+    auto consume = [&](int d, bool more) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(kTurn + 8));
+        else __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+        asm volatile("" ::: "memory");
+        u32x4 w[2][NW];
 #pragma unroll
-        for (int d = 0; d < kAhead; ++d) f[d] = load(s + d * kWaves);
-        for (; s + (2 * kAhead - 1) * kWaves < full; s += kAhead * kWaves)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int d = 0; d < kAhead; ++d) {
-                mul(f[d]);
-                f[d] = load(s + (d + kAhead) * kWaves);
+            for (int i = 0; i < NW; ++i) w[h][i] = mine[d * (kTurn * 64) + at[i] + ((h * 4 + kc) ^ (at[i] / 8 & 7))];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) mul(w[h], q[d][h]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // While the turn after the next exists, every turn asks for one: the number of requests in flight is known, and a turn
+    // waits for its own alone.  A wave reads only what it has asked for itself.
+    int s = begin + wave;
+    if (s + 3 * kWaves < full) {
+        request(s, 0);
+        request(s + kWaves, 1);
+        for (; s + 3 * kWaves < full; s += 2 * kWaves)
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                consume(d, true);
+                request(s + (d + 2) * kWaves, d);
             }
-#pragma unroll
-        for (int d = 0; d < kAhead; ++d) mul(f[d]);
-        s += kAhead * kWaves;
+        consume(0, true);
+        consume(1, false);
+        s += 2 * kWaves;
     }
-#pragma unroll
-    for (int d = 0; d < kAhead; ++d)
-        if (s + d * kWaves < full) f[d] = load(s + d * kWaves);
-#pragma unroll
-    for (int d = 0; d < kAhead; ++d)
-        if (s + d * kWaves < full) mul(f[d]);
-    s += kAhead * kWaves;
-    for (; s < full; s += kWaves) mul(load(s));
-    if (full * 128 < a.k && wave == full % kWaves) {       // the end of K; the codes are padded with zeros to whole 64
-        Frags e;
+    if (s < full) request(s, 0);
+    if (s + kWaves < full) request(s + kWaves, 1);
+    if (s < full) consume(0, s + kWaves < full);
+    if (s + 2 * kWaves < full) request(s + 2 * kWaves, 0);
+    if (s + kWaves < full) consume(1, s + 2 * kWaves < full);
+    if (s + 2 * kWaves < full) consume(0, false);
+    if (last && full * 128 < a.k && wave == (full - begin) % kWaves) {       // the end of K; the codes are padded with zeros to whole 64
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = full * 128 + h * 64;
+            u32x4 w[NW], e[4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) e.w[h][i] = weight_chunk(wp[i] - kc * 16, k + kc * 16, a.k, true);
+            for (int i = 0; i < NW; ++i) w[i] = weight_chunk(wb + min(at[i] / 8, most) * a.ldw, k + kc * 16, a.k, true);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e.q[h][i] = k < a.k ? qp[i][(long long)(k / 16) * a.ldq] : u32x4{0u, 0u, 0u, 0u};
+            for (int i = 0; i < 4; ++i) e[i] = k < a.k ? *(const u32x4 *)(qb + (long long)(k / 16) * a.ldq * 16 + qo[i]) : u32x4{0u, 0u, 0u, 0u};
+            mul(w, e);
         }
-        mul(e);
     }
-#pragma unroll
-    for (int i = 0; i < NR; ++i)
-#pragma unroll
-        for (int j = 0; j < NC; ++j) sums[wave][i * NC + j][lane] = acc[i][j];
     __syncthreads();
-    // a wave finishes one pair of row tiles and one column tile: four of them, the other waves are done
-    constexpr int T = 2, kParts = NR / T * NC;
-    static_assert(kParts == 4, "64 x 32");
-    if (wave >= kParts) return;
-    const int i0 = wave / NC * T, j = wave % NC;
-    int v[T][4] = {};
-    for (int w = 0; w < kWaves; ++w)
+    // the waves' sums meet in LDS, eight tiles at a time; a wave finishes two row tiles of one column tile
+    constexpr int T = 2, kRows = 8 / NC, kRounds = NR / kRows, kParts = kRows / T * NC;
+    static_assert(kParts == 4, "four waves finish a round, the other four the next one");
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        if (r) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) sums[wave][i * NC + j][lane] = acc[r * kRows + i][j];
+        __syncthreads();
+        const int part = wave - r * kParts;
+        if (part < 0 || part >= kParts) continue;
+        const int i0 = part / NC * T, j = part % NC;
+        i32x4 v[T] = {};
+        for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+            for (int i = 0; i < T; ++i) v[i] += sums[w][(i0 + i) * NC + j][lane];
+        const int col = c0 + j * 16 + r16;
+        if (col >= cols) continue;
 #pragma unroll
         for (int i = 0; i < T; ++i) {
-            const i32x4 p = sums[w][(i0 + i) * NC + j][lane];
+            const int row0 = r0 + (r * kRows + i0) * 16 + (PAIRS ? kc * 8 + i * 4 : i * 16 + kc * 4);
+            if (PART) {
+                int *to = a.part + ((long long)split * cols + col) * rows + row0;
+                if (row0 + 4 <= rows && (rows & 3) == 0) *(i32x4 *)to = v[i];
+                else
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] += p[e];
+                    for (int e = 0; e < 4; ++e)
+                        if (row0 + e < rows) to[e] = v[i][e];
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = row0 + e;
+                if (row >= rows) continue;
+                const int t = NCHW ? row : col, n = NCHW ? col : row;
+                store_one<DT>(a.y, out_base<NCHW>(a, t) + (NCHW ? (long long)n * a.plane : n),
+                              finished(a, v[i][e], a.scale[t], a.w_scale[n], a.bias ? a.bias[n] : 0.f));
+            }
         }
-    const int col = c0 + j * 16 + r16;
-    if (col >= cols) return;
-#pragma unroll
-    for (int i = 0; i < T; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = r0 + i0 * 16 + (PAIRS ? kc * 8 + i * 4 + e : i * 16 + kc * 4 + e);
-            if (row >= rows) continue;
-            const int t = NCHW ? row : col, n = NCHW ? col : row;
-            store_one<DT>(a.y, out_base<NCHW>(a, t) + (NCHW ? (long long)n * a.plane : n),
-                          finished(a, v[i][e], a.scale[t], a.w_scale[n], a.bias ? a.bias[n] : 0.f));
-        }
+    }
 }
 
 // Up to 16 tokens: a wave per channel, the weights read once, straight from the caller's rows, 16 bytes per lane and turn;
@@ -842,7 +868,7 @@ constexpr int kFusedTokens = 4, kGemvTokens = 16, kDirectTokens = 512;
 constexpr size_t kFusedLds = 64512;       // with the maxima within the 64 KiB that need no attribute
 enum { kFused, kGemv, kDirect, kTiles };
 
-// wide: the weights' rows start on 16 bytes (the sizes are the same either way)
+// wide: the weights' rows start on 16 bytes, and 64 of them lie within 32-bit offsets
 Plan plan_of(const ddcn_int8_geom *g, long long tokens, bool wide)
 {
     Plan p = {};
@@ -855,21 +881,42 @@ Plan plan_of(const ddcn_int8_geom *g, long long tokens, bool wide)
         p.q_bytes = p.scale_bytes = 0;
         return p;
     }
-    p.how = tokens <= kGemvTokens ? kGemv : tokens <= kDirectTokens && wide ? kDirect : kTiles;
-    if (p.how == kGemv) return p;
-    p.w_bytes = round_up((size_t)(chunks * 16 * g->channels), 256);
+    p.splits = 1;
+    if (tokens <= kGemvTokens) {
+        p.how = kGemv;
+        return p;
+    }
+    p.how = kTiles;
     // 128 x 128 tiles, four workgroups on a CU: 18818 x 2048 x 512 takes 28 us, 32768 x 2048 x 512 37 us (256 x 256 with
     // one workgroup on a CU: 52 and 39; 256 x 128: 35 and 40).  Smaller ones where those leave a quarter of the CUs idle.
-    long long tiles = ceil_div(tokens, 128) * ceil_div(g->channels, 128);
-    p.small = tiles < kCUs * 3 / 4;
-    if (p.small) tiles = ceil_div(tokens, 64) * ceil_div(g->channels, 64);
+    const long long wide_tiles = ceil_div(tokens, 128) * ceil_div(g->channels, 128);
+    const long long quarters = ceil_div(tokens, 64) * ceil_div(g->channels, 64);
+    p.small = wide_tiles < kCUs * 3 / 4;
+    const long long tiles = p.small ? quarters : wide_tiles;
     // K is split where the tiles leave CUs without work, into a power of two of pieces of 8 steps at least; long pieces once
-    // more, for a second workgroup on the CU (1024 tokens x 12544 x 1024: 56 -> 42 us with the sums of the two halves;
-    // 1024 x 1024 x 1024 would take 14 instead of 8)
-    long long splits = 1;
-    while (steps / (2 * splits) >= (tiles * splits < kCUs ? 8 : 32) && tiles * splits < 2 * kCUs) splits *= 2;
-    p.steps_per = (int)ceil_div(steps, splits);
-    p.splits = (int)ceil_div(steps, p.steps_per);
+    // more, for a second workgroup on the CU (1024 tokens x 12544 x 1024, rows at odd addresses: 56 -> 42 us with the sums
+    // of the two halves; 1024 x 1024 x 1024 would take 14 instead of 8)
+    long long pieces = 1;
+    while (steps / (2 * pieces) >= (tiles * pieces < kCUs ? 8 : 32) && tiles * pieces < 2 * kCUs) pieces *= 2;
+    // Direct: up to 512 tokens (512 x 2048 x 512: 7.7 us, tiles 8.5 + 3.6 and the weights' repacking; 512 x 25088 x 4096: 101,
+    // tiles 103 at twice the tokens, and 42 of repacking), and where tiles would split K but the direct kernel's fit the
+    // CUs (1024 x 12544 x 1024: 27, tiles 37 + 5 + 4; without the split tiles win: 2048 x 2048 x 512 12.5, direct 13.2).
+    const bool direct = wide && (tokens <= kDirectTokens || (pieces > 1 && quarters <= kCUs));
+    if (direct) {
+        p.how = kDirect;
+        // Its K is split from 32 turns of 128 k on where there are CUs for it, into pieces of 8 turns at least: 300 x 12544 x
+        // 1024 11.5 + 4 us (whole 22), 64 x 4096 x 1024 6 + 3.4 (whole 10.5), but 64 x 2048 x 512 5.9 + 2.9 (whole 7.6).
+        // Otherwise 32 channels to a workgroup instead of 64 where there are too few tiles.
+        const long long turns = g->k / 128;
+        pieces = turns < 32 ? 1 : kCUs / quarters < turns / 8 ? kCUs / quarters : turns / 8;
+        p.small = pieces < 2 && quarters < kCUs * 3 / 4;
+        if (pieces > 1) p.steps_per = (int)ceil_div(turns, pieces);
+        if (pieces > 1) p.splits = (int)ceil_div(turns, p.steps_per);
+    } else {
+        p.w_bytes = round_up((size_t)(chunks * 16 * g->channels), 256);
+        p.steps_per = (int)ceil_div(steps, pieces);
+        p.splits = (int)ceil_div(steps, p.steps_per);
+    }
     if (p.splits > 1) p.part_bytes = round_up((size_t)p.splits * tokens * g->channels * sizeof(int), 256);
     return p;
 }
@@ -916,14 +963,23 @@ template <int DT, bool NCHW, bool PART> int launch_gemm(const Int8Args &a, const
     if (!p.small) return launch_tiles<DT, NCHW, PART, 2, 2, 2>(a, s);
     return launch_tiles<DT, NCHW, PART, 1, 1, 4>(a, s);
 }
+template <int DT, bool NCHW, bool PART, int NW> int launch_direct(const Int8Args &a, hipStream_t s)
+{
+    constexpr int kLds = NW * 32768, kChannels = NW * 16;
+    static std::atomic<uint64_t> done{0};
+    if (!raise_lds_limit((const void *)direct8_kernel<DT, NCHW, PART, NW>, kLds, done)) return fail(DDCN_ERR_LAUNCH, "int8 product: LDS limit");
+    const long long grid = ceil_div(a.tokens, 64) * ceil_div(a.channels, kChannels) * a.splits;
+    direct8_kernel<DT, NCHW, PART, NW><<<(unsigned)grid, 512, kLds, s>>>(a);
+    return check_launch("int8 product");
+}
 template <int DT, bool NCHW> int launch_product(const Int8Args &a, const Plan &p, hipStream_t s)
 {
     const unsigned waves = (unsigned)ceil_div(a.channels, 4);
     if (p.how == kGemv) gemv8_kernel<DT, DDCN_F32, NCHW, 16, false><<<waves, 256, 0, s>>>(a);
-    if (p.how == kDirect) direct8_kernel<DT, NCHW><<<(unsigned)(ceil_div(a.tokens, 64) * ceil_div(a.channels, 32)), 512, 0, s>>>(a);
-    if (p.how != kTiles) return check_launch("int8 product");
+    if (p.how == kGemv) return check_launch("int8 product");
+    if (p.splits == 1 && p.how == kDirect) return p.small ? launch_direct<DT, NCHW, false, 2>(a, s) : launch_direct<DT, NCHW, false, 4>(a, s);
     if (p.splits == 1) return launch_gemm<DT, NCHW, false>(a, p, s);
-    const int rc = launch_gemm<DDCN_F32, NCHW, true>(a, p, s);
+    const int rc = p.how == kDirect ? launch_direct<DDCN_F32, NCHW, true, 4>(a, s) : launch_gemm<DDCN_F32, NCHW, true>(a, p, s);
     if (rc != DDCN_OK) return rc;
     finish_kernel<DT, NCHW><<<(unsigned)ceil_div((long long)a.tokens * a.channels, 256), 256, 0, s>>>(a, p.splits);
     return check_launch("int8 finish");
@@ -977,7 +1033,9 @@ size_t ddcn_int8_workspace_bytes(const ddcn_int8_geom *g)
 {
     if (check(g, true) != DDCN_OK || !tokens_of(g)) return 0;
     const long long tokens = tokens_of(g);
-    return plan_of(g, tokens < kPassTokens ? tokens : kPassTokens, true).bytes();
+    const long long pass = tokens < kPassTokens ? tokens : kPassTokens;
+    const size_t aligned = plan_of(g, pass, true).bytes(), other = plan_of(g, pass, false).bytes();
+    return aligned > other ? aligned : other;
 }
 
 int ddcn_int8_product(const void *x, const void *weight, const float *weight_scale, const float *bias, void *y,
@@ -999,7 +1057,7 @@ int ddcn_int8_product(const void *x, const void *weight, const float *weight_sca
     const long long total = tokens_of(g);
     for (a.t0 = 0; a.t0 < total; a.t0 += kPassTokens) {    // (later passes fit the first one's workspace)
         a.tokens = (int)(total - a.t0 < kPassTokens ? total - a.t0 : kPassTokens);
-        const Plan p = plan_of(g, a.tokens, (((uintptr_t)weight | (uintptr_t)g->ldw) & 15) == 0);
+        const Plan p = plan_of(g, a.tokens, (((uintptr_t)weight | (uintptr_t)g->ldw) & 15) == 0 && g->ldw < (1LL << 25));
         if (p.how == kFused) {
             rc = g->nchw ? run_fused<true>(a, g->dtype, g->out_dtype, (hipStream_t)stream) : run_fused<false>(a, g->dtype, g->out_dtype, (hipStream_t)stream);
             if (rc != DDCN_OK) return rc;

@@ -72,6 +72,19 @@ def test_linear_over_types(dtype, out, tokens, k, n):
         _close(y, want, tol, TYPES[out])
 
 
+@pytest.mark.parametrize("tokens,k,n", [(17, 4096, 64), (70, 4097, 33), (65, 4112, 200), (300, 12544, 130), (64, 9999, 257), (130, 5136, 70),
+                                        (600, 2048, 100), (1000, 6000, 700), (513, 1040, 65), (20, 1300, 13000)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nchw", [False, True])
+def test_long_sums_over_few_tokens(tokens, k, n, dtype, nchw):
+    """K split between workgroups, with ends that are no whole turn; the tokens as rows, and as the pixels of a map."""
+    x = _make((tokens, k), TYPES[dtype], k + n)
+    wq, ws, b = _weights(n, k, n)
+    want, tol = ref.product(_np(x), _np(wq), _np(ws), _np(b))
+    y = pkg.int8_conv1x1(x.t().contiguous().view(1, k, 1, tokens), wq, ws, b).view(n, tokens).t() if nchw else pkg.int8_linear(x, wq, ws, b)
+    _close(y, want, tol, TYPES[dtype])
+
+
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("images,c,co,h,w", [(1, 3, 64, 7, 5), (2, 64, 64, 9, 11), (1, 130, 40, 1, 1), (3, 17, 3, 13, 1),
                                              (2, 256, 300, 16, 17), (1, 1000, 19, 5, 70), (4, 1, 2, 3, 3)])
