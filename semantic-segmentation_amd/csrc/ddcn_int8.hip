@@ -155,14 +155,19 @@ template <int DT> __device__ __forceinline__ void load_16(const Int8Args &a, lon
     }
 }
 
-// sk == 1: W waves per token, 16 consecutive values per lane and turn, up to I turns held in registers (more are read again)
-template <int DT, int W, int I> __global__ __launch_bounds__(256) void prepare_rows_kernel(const Int8Args a)
+// sk == 1, a row of x per token: 16 consecutive values per lane and turn, up to I turns held in registers (more are read
+// again).  W > 1: W waves per token.  W == 1: 2^lanes_log lanes per token (all 64 if I > 1), 512 threads, whose codes meet in
+// LDS and leave as whole lines -- eight tokens a workgroup at least (60000 x 2048 bf16: 63 us, 5.8 TB/s; a wave storing the 16
+// bytes of each chunk by itself 93; 60000 x 64: 4.6 us, 24 with a wave for each token).
+template <int DT, int W, int I> __global__ __launch_bounds__(W == 1 ? 512 : 64 * W) void prepare_rows_kernel(const Int8Args a, int lanes_log)
 {
     if ((int)blockIdx.x >= a.prep_blocks) return repack_weights(a, blockIdx.x - a.prep_blocks, gridDim.x - a.prep_blocks);
+    if (W > 1 || I > 1) lanes_log = 6;
+    const int lanes = 1 << lanes_log, tokens = W == 1 ? 512 >> lanes_log : 1, turn = lanes * W;        // turn: chunks of one
     __shared__ unsigned tops[4];
-    constexpr int kTurn = 64 * W;                          // chunks of a turn
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t = xcd_logical(blockIdx.x, a.prep_blocks) * (4 / W) + wave / W, first = (wave % W) * 64 + lane;
+    __shared__ u32x4 lines[W == 1 ? I * 512 : 1];
+    const int j = W == 1 ? threadIdx.x >> lanes_log : 0, first = threadIdx.x & (turn - 1);
+    const int t_first = xcd_logical(blockIdx.x, a.prep_blocks) * tokens, t = t_first + j;
     const bool live = t < a.tokens;
     const long long base = live ? token_base(a, t) : 0;
     constexpr int kAlign = DT == DDCN_F32 ? 4 : 8;
@@ -172,37 +177,51 @@ template <int DT, int W, int I> __global__ __launch_bounds__(256) void prepare_r
     if (live) {
 #pragma unroll
         for (int i = 0; i < I; ++i)
-            if (first + i * kTurn < a.chunks) load_16<DT>(a, base, (first + i * kTurn) * 16, vec, x[i]);
+            if (first + i * turn < a.chunks) load_16<DT>(a, base, (first + i * turn) * 16, vec, x[i]);
 #pragma unroll
         for (int i = 0; i < I; ++i)
-            if (first + i * kTurn < a.chunks)
+            if (first + i * turn < a.chunks)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) top = max(top, bits_of(x[i][e]));
-        for (int c = first + I * kTurn; c < a.chunks; c += kTurn) {
+        for (int c = first + I * turn; c < a.chunks; c += turn) {
             float z[16];
             load_16<DT>(a, base, c * 16, vec, z);
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = max(top, bits_of(z[e]));
         }
     }
-    for (int d = 32; d; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
+    for (int d = lanes >> 1; d; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
     if (W > 1) {
-        if (lane == 0) tops[wave] = top;
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
         __syncthreads();
         top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
     }
-    if (!live) return;
     float scale, factor;
     token_scale(top, scale, factor);
+    if (live && first == 0) a.scale[a.q_rows ? a.t0 + t : t] = scale;
+    if (W == 1 && !a.q_rows) {
+        // chunk c of token j in place j ^ (c % 8) of its line
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int c = first + i * turn;
+            if (live && c < a.chunks) lines[c * tokens + (j ^ (c & 7))] = pack16(x[i], factor);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.chunks * tokens; i += 512) {
+            const int c = i >> (9 - lanes_log), to = t_first + ((i & (tokens - 1)) ^ (c & 7));
+            if (to < a.tokens) a.q[(long long)c * a.ldq + to] = lines[i];
+        }
+        return;
+    }
+    if (!live) return;
 #pragma unroll
     for (int i = 0; i < I; ++i)
-        if (first + i * kTurn < a.chunks) store_chunk(a, t, first + i * kTurn, pack16(x[i], factor));
-    for (int c = first + I * kTurn; c < a.chunks; c += kTurn) {
+        if (first + i * turn < a.chunks) store_chunk(a, t, first + i * turn, pack16(x[i], factor));
+    for (int c = first + I * turn; c < a.chunks; c += turn) {
         float z[16];
         load_16<DT>(a, base, c * 16, vec, z);
         store_chunk(a, t, c, pack16(z, factor));
     }
-    if (first == 0) a.scale[a.q_rows ? a.t0 + t : t] = scale;
 }
 
 // Sixteen values of a chunk as they are stored: 16-bit ones in pairs
@@ -926,12 +945,17 @@ template <int DT> void launch_prepare(Int8Args &a, bool repack, hipStream_t s)
     // repacking: a wave moves 64 chunks; enough workgroups to take no longer than the tokens do
     const int extra = repack ? (int)(ceil_div((long long)a.channels * a.chunks, 64 * 16) < 4096 ? ceil_div((long long)a.channels * a.chunks, 64 * 16) : 4096) : 0;
     if (a.sk == 1) {
-        const bool many = a.chunks > 128;                  // more than 2048 values: four waves per token
-        a.prep_blocks = (int)ceil_div(a.tokens, many ? 1 : 4);
+        // four waves per token for more than 4096 values, and for more than 1024 where tokens are few (300 x 2048: 3.9 us,
+        // 4.4 with one wave each; 2000 x 2048: 8.9, 7.5 with one; 18818 x 4096: 59, 46 with one)
+        const bool many = a.chunks > 256 || (a.chunks > 64 && a.tokens <= 4 * kCUs);
+        int lanes_log = 2;                                 // whole K steps are four chunks
+        while (lanes_log < 6 && a.chunks > 1 << lanes_log) ++lanes_log;
+        a.prep_blocks = (int)ceil_div(a.tokens, many ? 1 : 512 >> lanes_log);
         const unsigned grid = (unsigned)(a.prep_blocks + extra);
-        if (many) prepare_rows_kernel<DT, 4, 4><<<grid, 256, 0, s>>>(a);
-        else if (a.chunks > 64) prepare_rows_kernel<DT, 1, 2><<<grid, 256, 0, s>>>(a);
-        else prepare_rows_kernel<DT, 1, 1><<<grid, 256, 0, s>>>(a);
+        if (many) prepare_rows_kernel<DT, 4, 4><<<grid, 256, 0, s>>>(a, 6);
+        else if (a.chunks > 128) prepare_rows_kernel<DT, 1, 4><<<grid, 512, 0, s>>>(a, 6);
+        else if (a.chunks > 64) prepare_rows_kernel<DT, 1, 2><<<grid, 512, 0, s>>>(a, 6);
+        else prepare_rows_kernel<DT, 1, 1><<<grid, 512, 0, s>>>(a, lanes_log);
     } else {
         a.prep_blocks = (int)ceil_div(a.tokens, 32);
         const unsigned grid = (unsigned)(a.prep_blocks + extra);

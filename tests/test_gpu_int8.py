@@ -59,6 +59,20 @@ def test_linear_over_sizes(tokens, k, n):
     _close(pkg.int8_linear(x, wq, ws, b), want, tol, torch.float32)
 
 
+@pytest.mark.parametrize("tokens,k", [(1030, 40), (1100, 100), (1029, 300), (1100, 1000), (1101, 1500), (2051, 2048), (1100, 3000), (1025, 4100)])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("shift", [0, 1])
+def test_many_tokens_of_any_length(tokens, k, dtype, shift):
+    """Rows rounded by a part of a wave, a wave and several, at aligned and other addresses."""
+    x = _make((tokens, k + shift), TYPES[dtype], k)[:, shift:]
+    wq, ws, b = _weights(70, k, 3)
+    want, tol = ref.product(_np(x), _np(wq), _np(ws), _np(b))
+    _close(pkg.int8_linear(x, wq, ws, b, out_dtype=torch.float32), want, tol, torch.float32)
+    q, s = pkg.quantize_int8(x)
+    wq_, ws_ = ref.quantize(_np(x))
+    assert np.array_equal(_np(q), wq_) and np.array_equal(_np(s), ws_)
+
+
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("out", sorted(TYPES))
 @pytest.mark.parametrize("tokens,k,n", [(1, 500, 96), (9, 12544, 40), (77, 500, 96), (700, 256, 520)])
