@@ -313,16 +313,14 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const signed char *m
 
 // ---------------------------------------------------------------- norm
 constexpr int kNormChunk = 8192;       // elements of a workgroup
-struct NormTensor {
-    const void *g;
-    long long n;
-    unsigned chunk0;
-    int dtype;
-};
-constexpr int kMaxNorm = 160;
+// 16 bytes a tensor, so that ResNet-50's 237 tensors fit one launch (62.6 us; two launches of 160 took 14.2 + 51.4 and a gap)
+constexpr int kMaxNorm = 254;
+constexpr unsigned kFirstChunk = 0x3FFFFFFFu;
 struct NormArgs {
-    NormTensor t[kMaxNorm];
-    double *partial;       // of this launch's first workgroup
+    const void *g[kMaxNorm];
+    unsigned n[kMaxNorm];          // at most 2^31
+    unsigned chunk0[kMaxNorm];     // first workgroup, and the element type in the two highest bits
+    double *partial;               // of this launch's first workgroup
     int count;
 };
 static_assert(sizeof(NormArgs) <= 4096, "kernel argument segment");
@@ -338,19 +336,19 @@ __device__ __forceinline__ double block_sum(double s, double *lds)
     return s;
 }
 
-template <int DT> __device__ __forceinline__ double chunk_square(const NormTensor &t, long long begin)
+template <int DT> __device__ __forceinline__ double chunk_square(const void *g, long long n, long long begin)
 {
     constexpr unsigned kMask = DT == DDCN_F32 ? 15u : 7u;
     constexpr int kAhead = 8;          // wide loads in flight
-    const bool vec = ((unsigned long long)t.g & kMask) == 0;
-    const long long end = min(t.n, begin + kNormChunk);
+    const bool vec = ((unsigned long long)g & kMask) == 0;
+    const long long end = min(n, begin + kNormChunk);
     double s[4] = {0., 0., 0., 0.};
-    if (vec && begin + kNormChunk <= t.n) {
+    if (vec && begin + kNormChunk <= n) {
 #pragma unroll
         for (int k = 0; k < kNormChunk / 1024; k += kAhead) {
             float x[kAhead][4];
 #pragma unroll
-            for (int l = 0; l < kAhead; ++l) load_four<DT>(t.g, begin + (k + l) * 1024 + threadIdx.x * 4, x[l]);
+            for (int l = 0; l < kAhead; ++l) load_four<DT>(g, begin + (k + l) * 1024 + threadIdx.x * 4, x[l]);
 #pragma unroll
             for (int l = 0; l < kAhead; ++l)
                 for (int e = 0; e < 4; ++e) s[e] = fma((double)x[l][e], (double)x[l][e], s[e]);
@@ -358,7 +356,7 @@ template <int DT> __device__ __forceinline__ double chunk_square(const NormTenso
     } else {
         for (long long i = begin + threadIdx.x * 4; i < end; i += 1024) {
             float x[4];
-            load_some<DT>(t.g, i, (int)min(end - i, 4LL), vec, x);
+            load_some<DT>(g, i, (int)min(end - i, 4LL), vec, x);
             for (int e = 0; e < 4; ++e) s[e] = fma((double)x[e], (double)x[e], s[e]);
         }
     }
@@ -371,14 +369,15 @@ __global__ __launch_bounds__(256) void norm_partial_kernel(const NormArgs a)
     // the last tensor whose first workgroup is not behind this one, 64 compared at once
     const int lane = threadIdx.x & 63;
     int j = -1;
-    for (int i = 0; i < 3; ++i) {
-        const unsigned c0 = lane + 64 * i < a.count ? a.t[min(lane + 64 * i, kMaxNorm - 1)].chunk0 : 0xFFFFFFFFu;
+    for (int i = 0; i < 4; ++i) {
+        const unsigned c0 = lane + 64 * i < a.count ? a.chunk0[min(lane + 64 * i, kMaxNorm - 1)] & kFirstChunk : 0xFFFFFFFFu;
         j += __popcll(__ballot(c0 <= blockIdx.x));
     }
-    const NormTensor &t = a.t[j];
-    const long long begin = (long long)(blockIdx.x - t.chunk0) * kNormChunk;
-    double s = t.dtype == DDCN_F32 ? chunk_square<DDCN_F32>(t, begin)
-               : t.dtype == DDCN_BF16 ? chunk_square<DDCN_BF16>(t, begin) : chunk_square<DDCN_F16>(t, begin);
+    const void *g = a.g[j];
+    const unsigned dtype = a.chunk0[j] >> 30;
+    const long long n = a.n[j], begin = (long long)(blockIdx.x - (a.chunk0[j] & kFirstChunk)) * kNormChunk;
+    double s = dtype == DDCN_F32 ? chunk_square<DDCN_F32>(g, n, begin)
+               : dtype == DDCN_BF16 ? chunk_square<DDCN_BF16>(g, n, begin) : chunk_square<DDCN_F16>(g, n, begin);
     s = block_sum(s, lds);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = s;
 }
@@ -554,27 +553,29 @@ int ddcn_grad_norm(int count, const unsigned long long *grads, const long long *
     NormArgs a;
     a.count = 0;
     long long chunks = 0, done = 0;
-    for (int i = 0; i <= count; ++i) {
-        const bool end = i == count;
-        const long long mine = end ? 0 : ceil_div(numels[i], kNormChunk);
-        if (a.count && (end || a.count == kMaxNorm || chunks + mine > kMaxGrid)) {
-            a.partial = (double *)workspace + done;
-            norm_partial_kernel<<<(unsigned)chunks, 256, 0, (hipStream_t)stream>>>(a);
-            const int rc = check_launch("grad_norm");
-            if (rc != DDCN_OK) return rc;
-            done += chunks;
-            a.count = 0;
-            chunks = 0;
+    auto launch = [&]() -> int {
+        if (!a.count) return DDCN_OK;
+        a.partial = (double *)workspace + done;
+        norm_partial_kernel<<<(unsigned)chunks, 256, 0, (hipStream_t)stream>>>(a);
+        done += chunks;
+        a.count = 0;
+        chunks = 0;
+        return check_launch("grad_norm");
+    };
+    for (int i = 0; i < count; ++i)
+        for (long long at = 0; at < numels[i]; at += 1LL << 31) {      // (whole chunks)
+            const long long n = numels[i] - at < (1LL << 31) ? numels[i] - at : 1LL << 31, mine = ceil_div(n, kNormChunk);
+            if (a.count == kMaxNorm || chunks + mine > kMaxGrid) {
+                const int rc = launch();
+                if (rc != DDCN_OK) return rc;
+            }
+            a.g[a.count] = (const void *)(grads[i] + at * (dtypes[i] == DDCN_F32 ? 4 : 2));
+            a.n[a.count] = (unsigned)n;
+            a.chunk0[a.count++] = (unsigned)chunks | (unsigned)dtypes[i] << 30;
+            chunks += mine;
         }
-        if (end) break;
-        if (!mine) continue;
-        NormTensor &t = a.t[a.count++];
-        t.g = (const void *)grads[i];
-        t.n = numels[i];
-        t.chunk0 = (unsigned)chunks;
-        t.dtype = dtypes[i];
-        chunks += mine;
-    }
+    const int rc = launch();
+    if (rc != DDCN_OK) return rc;
     norm_final_kernel<<<1, 1024, 0, (hipStream_t)stream>>>((const double *)workspace, done, out);
     return check_launch("grad_norm");
 }

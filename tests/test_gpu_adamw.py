@@ -534,3 +534,11 @@ def test_moments_of_more_elements_than_a_grid_has_room_for():
         a, b = callers.adamw_moments(m[at].clone(), v[at].clone(), sm[s].clone(), sv[s].clone())
         assert torch.equal(dm[at], a) and torch.equal(dv[at], b) and a.any() and b.any()
     assert not dm[512:4096].any() and not dv[-(1 << 20) - 1024:-1024].any()
+
+
+def test_grad_norm_of_more_than_2_31_elements():
+    g = torch.zeros((1 << 31) + 5000, dtype=torch.bfloat16, device=DEV)
+    small = torch.full((3,), 2.0, device=DEV)
+    for at in (0, 1 << 20, (1 << 31) - 1, 1 << 31, (1 << 31) + 4999):
+        g[at] = 3.0
+    assert float(callers.grad_norm([small, g, small])) == np.float32(np.sqrt(5 * 9 + 2 * 3 * 4))
