@@ -417,10 +417,10 @@ typedef struct ddcn_int8_geom {
 
 size_t ddcn_int8_workspace_bytes(const ddcn_int8_geom *g);
 /* weight: int8 [channels][ldw] (k of each row are read), weight_scale fp32 [channels], bias fp32 [channels] or NULL.
- * `workspace`: ddcn_int8_workspace_bytes(), 256-byte aligned. */
+ * `workspace`: ddcn_int8_workspace_bytes(), 256-byte aligned; 0 bytes and NULL for some calls of up to 4 tokens. */
 int ddcn_int8_product(const void *x, const void *weight, const float *weight_scale, const float *bias, void *y,
                       void *workspace, size_t workspace_bytes, const ddcn_int8_geom *g, void *stream);
-/* The rounding alone: q int8 [tokens][ldq] (ldq >= k; bytes from k to ldq are zeroed), scale fp32 [tokens]. */
+/* The rounding alone: q int8 [tokens][ldq] (k <= ldq <= k + 64; bytes from k to ldq are zeroed), scale fp32 [tokens]. */
 int ddcn_int8_quantize(const void *x, void *q, long long ldq, float *scale, const ddcn_int8_geom *g, void *stream);
 
 #ifdef __cplusplus

@@ -290,7 +290,8 @@ template <int DT> __device__ __forceinline__ u32x4 pack_raw(const Raw<DT> &r, fl
 
 // Any strides, lanes along the tokens: 32 tokens per workgroup; a wave takes two chunks of 16 channels at a time (one per
 // half), I such pairs held in registers as they came (more are read again).  16-bit values in pairs leave room for two
-// workgroups of 1024 on a CU: one loads while the other rounds and stores.
+// workgroups of 1024 on a CU: one loads while the other rounds and stores.  Bound by HBM: 32768 x 2048 bf16 in 48 us (201 MB,
+// 4.2 TB/s); two pixels to a load, 64 tokens to a workgroup takes 49, and more where pixels are few.
 template <int DT, int NT, int I> __global__ __launch_bounds__(NT, DT != DDCN_F32 && NT == 1024 ? 8 : 4) void prepare_map_kernel(const Int8Args a)
 {
     if ((int)blockIdx.x >= a.prep_blocks) return repack_weights(a, blockIdx.x - a.prep_blocks, gridDim.x - a.prep_blocks);
@@ -604,7 +605,7 @@ __global__ __launch_bounds__(128 * NWN, 4) void gemm8_kernel(const Int8Args a)
     }
 }
 
-// sums [split][columns][rows] -> y, in the order of y
+// sums [split][columns][rows] -> y, in the order of y (300 x 1024 in three pieces: 4.0 us, a launch and one round of latencies)
 template <int DT, bool NCHW> __global__ __launch_bounds__(256) void finish_kernel(const Int8Args a, int splits)
 {
     const int rows = NCHW ? a.tokens : a.channels, cols = NCHW ? a.channels : a.tokens;
@@ -771,7 +772,7 @@ template <int DT, bool NCHW, bool PART, int NW> __global__ __launch_bounds__(512
 // Up to 16 tokens: a wave per channel, the weights read once, straight from the caller's rows, 16 bytes per lane and turn;
 // the codes of a chunk lie next to each other.  FUSED (up to TOK = 4 tokens whose codes fit LDS): every workgroup rounds the
 // tokens itself while its first weights are on their way -- one launch, no workspace; the rounding is repeated by every
-// workgroup, from the caches.
+// workgroup, from the caches.  1 x 12544 x 1024 fp32: 8.1 us (two launches 4.0 + 5.3), of which 2.5 would be the weights' bytes.
 template <int DT, int IN, bool NCHW, int TOK, bool FUSED> __global__ __launch_bounds__(256) void gemv8_kernel(const Int8Args a)
 {
     extern __shared__ u32x4 codes[];                       // FUSED: [chunk][TOK]

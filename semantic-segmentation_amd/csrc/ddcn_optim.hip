@@ -235,7 +235,9 @@ __device__ __forceinline__ void update_block(const AdamwArgs &a, const Place &w,
 }
 
 // U blocks per wave, one after the other in the arena; where all of them are whole, every load is issued before the first
-// result is needed
+// result is needed.  Every byte moves once.  fp32 moments, 28 bytes an element: bound by HBM, 39.6 M elements in 185 us, 6.0
+// TB/s.  8-bit ones, 16 bytes an element: 106 us for the same, 6.0 TB/s.  With bf16 parameters too, 10 bytes an element, its
+// 100 VALU instructions -- decoding, hash, two roots and their rounding -- bound it: 45 M elements in 113 us, 4.0 TB/s.
 template <int DT, int BITS, int U>
 __global__ __launch_bounds__(64 * kWaves) void adamw_kernel(const AdamwArgs a)
 {
@@ -291,6 +293,7 @@ __global__ __launch_bounds__(64 * kWaves) void adamw_kernel(const AdamwArgs a)
     }
 }
 
+// Bound by HBM: 2 bytes in and 8 out, 48 M elements in 75 us, 6.5 TB/s
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const signed char *m, const unsigned char *v, const float *sm,
                                                             const float *sv, float *om, float *ov, long long quads)
 {
@@ -363,6 +366,9 @@ template <int DT> __device__ __forceinline__ double chunk_square(const void *g, 
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
+// Sums in fp64 (the adds hide behind the loads), a workgroup a chunk, their sums in a fixed order by one workgroup: no
+// atomics.  Read-only: 48 M fp32 elements in 42 us where they come from HBM alone, 62 right after a step, whose writes
+// are then still leaving the last-level cache.
 __global__ __launch_bounds__(256) void norm_partial_kernel(const NormArgs a)
 {
     __shared__ double lds[4];
