@@ -8,7 +8,6 @@ i - 1 (`adamw_arena` gives the length).  In 8 bits `exp_avg` is int8, `exp_avg_s
 """
 import ctypes
 from array import array
-from operator import attrgetter
 
 import torch
 
@@ -16,26 +15,19 @@ from ..dcn import _lib
 
 BLOCK = 256
 _Tensor = torch.Tensor
-_dtype_of = attrgetter("dtype")
 
 
 def _address(a):
     return ctypes.c_void_p(a.buffer_info()[0]) if len(a) else None
 
 
-def _one_device(tensors, name):
-    """Index of the GPU that every tensor lives on."""
-    where = set(map(_Tensor.get_device, tensors))
-    if -1 in where:
+def _check_device(device, name):
+    """The common GPU of tensors that `describe` has seen."""
+    if device == -1:
         raise NotImplementedError
-    if len(where) > 1:
+    if device == -2:
         raise RuntimeError("ddcn: %s are on more than one device" % name)
-    return where.pop()
-
-
-def _all_contiguous(tensors):
-    # (a sparse tensor raises a RuntimeError of torch's own here)
-    return all(map(_Tensor.is_contiguous, tensors))
+    return device
 
 
 def _dense(t):
@@ -48,8 +40,8 @@ def _same_order(a, b):
     return a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous())
 
 
-def _arena_of(numels):
-    n = _lib.lib().ddcn_adamw_arena(len(numels), _address(numels))
+def _arena_of(count, numels):
+    n = _lib.lib().ddcn_adamw_arena(count, numels)
     if n < 0:
         _lib.check(n)
     return n
@@ -57,7 +49,8 @@ def _arena_of(numels):
 
 def adamw_arena(params):
     """Elements of the arena that holds one moment of `params`."""
-    return _arena_of(array("q", map(_Tensor.numel, params)))
+    numels = array("q", map(_Tensor.numel, params))
+    return _arena_of(len(numels), _address(numels))
 
 
 def grad_norm(grads):
@@ -66,21 +59,20 @@ def grad_norm(grads):
     grads = [g for g in grads if g is not None]
     if not grads:
         raise RuntimeError("ddcn: grad_norm needs at least one gradient")
-    dev = _one_device(grads, "gradients")
-    if not _all_contiguous(grads) and not all(map(_dense, grads)):
+    pointers, numels, dtypes, dev, dtype, contiguous, _, _ = _lib.tensors().describe(grads)
+    _check_device(dev, "gradients")
+    if not contiguous and not all(map(_dense, grads)):
         raise RuntimeError("ddcn: gradient tensors have to be contiguous (or channels-last)")
-    try:
-        dtypes = array("i", map(_lib.ELEMENT_TYPES.__getitem__, map(_dtype_of, grads)))
-    except KeyError as e:
-        raise RuntimeError("ddcn: %s gradients are not supported (float32, float16, bfloat16)" % e) from None
-    pointers, numels = array("Q", map(_Tensor.data_ptr, grads)), array("q", map(_Tensor.numel, grads))
+    if dtype == -1:
+        other = next(g.dtype for g in grads if g.dtype not in _lib.ELEMENT_TYPES)
+        raise RuntimeError("ddcn: %s gradients are not supported (float32, float16, bfloat16)" % other)
     L = _lib.lib()
-    nbytes = L.ddcn_grad_norm_workspace_bytes(len(grads), _address(numels))
+    nbytes = L.ddcn_grad_norm_workspace_bytes(len(grads), numels)
     with _lib.on_device(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device)
         out = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        _lib.check(L.ddcn_grad_norm(len(grads), _address(pointers), _address(numels), _address(dtypes), _lib.ptr(out),
-                                    _lib.ptr(ws), nbytes, _lib.stream_of(dev)))
+        _lib.check(L.ddcn_grad_norm(len(grads), pointers, numels, dtypes, _lib.ptr(out), _lib.ptr(ws), nbytes,
+                                    _lib.stream_of(dev)))
     return out
 
 
@@ -115,27 +107,29 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
         raise RuntimeError("ddcn: %d parameters but %d gradients" % (len(params), len(grads)))
     if not params:
         return
-    dtype = params[0].dtype
-    given = [g for g in grads if g is not None]
-    mine = params if len(given) == len(grads) else [p for p, g in zip(params, grads) if g is not None]
-    dev = _one_device(params + given + ([grad_norm] if grad_norm is not None else []), "parameters and gradients")
-    if dtype not in _lib.ELEMENT_TYPES:
-        raise RuntimeError("ddcn: %s parameters are not supported (float32, float16, bfloat16)" % dtype)
-    if set(map(_dtype_of, params)) | set(map(_dtype_of, given)) != {dtype}:
-        raise RuntimeError("ddcn: the parameters and gradients of one step must share a dtype (%s)" % dtype)
-    if not _all_contiguous(mine) or not _all_contiguous(given):
-        if not all(_same_order(p, g) and _dense(p) for p, g in zip(mine, given)):
+    describe = _lib.tensors().describe
+    pointers, numels, _, dev, code, contiguous, distinct, count = describe(params)
+    gradients, grad_numels, _, grad_dev, grad_code, grad_contiguous, _, given = describe(grads)
+    if count < len(params):
+        raise RuntimeError("ddcn: a parameter is None")
+    if -1 in (dev, grad_dev) or (grad_norm is not None and not grad_norm.is_cuda):
+        raise NotImplementedError
+    if dev == -2 or (given and grad_dev != dev) or (grad_norm is not None and grad_norm.get_device() != dev):
+        raise RuntimeError("ddcn: parameters and gradients are on more than one device")
+    if params[0].dtype not in _lib.ELEMENT_TYPES:
+        raise RuntimeError("ddcn: %s parameters are not supported (float32, float16, bfloat16)" % params[0].dtype)
+    if code < 0 or (given and grad_code != code):
+        raise RuntimeError("ddcn: the parameters and gradients of one step must share a dtype (%s)" % params[0].dtype)
+    if given < len(grads) or not contiguous or not grad_contiguous or numels != grad_numels:
+        wrong = _lib.tensors().alike(params, grads)
+        if wrong == 1:
             raise RuntimeError("ddcn: parameters have to be contiguous (or channels-last), gradients in the same order")
-    numels = array("q", map(_Tensor.numel, params))
-    if array("q", map(_Tensor.numel, given)) != (numels if mine is params else array("q", map(_Tensor.numel, mine))):
-        raise RuntimeError("ddcn: a gradient has another number of elements than its parameter")
-    pointers = array("Q", map(_Tensor.data_ptr, params))
-    if len(set(pointers)) != len(pointers):            # (empty tensors may share an address)
-        starts = [a for a, n in zip(pointers, numels) if n]
-        if len(set(starts)) != len(starts):
-            raise RuntimeError("ddcn: a parameter is listed twice")
+        if wrong == 2:
+            raise RuntimeError("ddcn: a gradient has another number of elements than its parameter")
+    if not distinct:
+        raise RuntimeError("ddcn: a parameter is listed twice")
     L = _lib.lib()
-    arena = _arena_of(numels)
+    arena = _arena_of(len(params), numels)
     bits = 8 if exp_avg.dtype == torch.int8 else 32
     _check_state("exp_avg", exp_avg, torch.int8 if bits == 8 else torch.float32, arena, dev)
     _check_state("exp_avg_sq", exp_avg_sq, torch.uint8 if bits == 8 else torch.float32, arena, dev)
@@ -156,24 +150,19 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
         if len(steps) != len(params):
             raise RuntimeError("ddcn: %d parameters but %d step numbers" % (len(params), len(steps)))
     hyper = _lib.AdamwHyper(lr, betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, step,
-                            _lib.ELEMENT_TYPES[dtype], bits, int(seed) & 0xFFFFFFFF)
-    if mine is params:
-        gradients = array("Q", map(_Tensor.data_ptr, grads))
-    else:
-        gradients = array("Q", [0 if g is None else g.data_ptr() for g in grads])
+                            code, bits, int(seed) & 0xFFFFFFFF)
     with _lib.on_device(dev):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("ddcn: adamw_step cannot be captured into a HIP graph: a replay would repeat the step "
                                "number, the learning rate and the seed of the capture")
-        _lib.check(L.ddcn_adamw_step(len(params), _address(pointers), _address(gradients), _address(numels),
+        _lib.check(L.ddcn_adamw_step(len(params), pointers, gradients, numels,
                                      None if steps is None else _address(steps), _lib.ptr(exp_avg),
                                      _lib.ptr(exp_avg_sq), _lib.ptr(exp_avg_scale), _lib.ptr(exp_avg_sq_scale),
                                      _lib.ptr(grad_norm), hyper, _lib.stream_of(dev)))
     # the kernels write behind autograd's back: a backward pass that saved one of these must notice
-    changed = mine + [exp_avg, exp_avg_sq] + ([exp_avg_scale, exp_avg_sq_scale] if bits == 8 else [])
-    if torch.is_inference_mode_enabled() or exp_avg.is_inference():      # such tensors keep no versions
-        changed = [t for t in changed if not t.is_inference()]
-    torch.autograd.graph.increment_version(changed)
+    changed = _lib.tensors().changed
+    changed(params, grads)
+    changed([exp_avg, exp_avg_sq] if bits == 32 else [exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale])
 
 
 def adamw_moments(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
@@ -278,7 +267,7 @@ class AdamW(torch.optim.Optimizer):
             if all(x is None for x in gs):
                 continue
             group, arena, state = self.param_groups[g], self._arena(g, dtype, params), self.state
-            if not _all_contiguous(params) or not _all_contiguous([x for x in gs if x is not None]):
+            if _lib.tensors().alike(params, gs) == 1:
                 gs = [x if x is None or _same_order(x, p) else torch.empty_like(p).copy_(x) for p, x in zip(params, gs)]
             steps = [state[p]["step"] + (x is not None) for p, x in zip(params, gs)]
             same = steps[0] if steps.count(steps[0]) == len(steps) else None

@@ -5,6 +5,7 @@ This is the counterpart of the reference's `from . import deform_conv_cuda`
 library is missing the import fails loudly.
 """
 import ctypes
+import importlib.util
 import os
 
 import torch  # noqa: F401  (imported first so that the library binds to torch's HIP runtime)
@@ -157,6 +158,24 @@ def lib():
             fn.restype = _RESTYPES.get(name, ctypes.c_int)
         _lib = handle
     return _lib
+
+
+_tensors = None
+
+
+def tensors():
+    """The CPython module of csrc/ddcn_tensors.cpp (lists of tensors for the optimizer), built with the library."""
+    global _tensors
+    if _tensors is None:
+        path = os.path.join(_PKG, "lib", "_ddcn_tensors.so")
+        if not os.path.exists(path):
+            raise ImportError("_ddcn_tensors.so not found at %s: build it with `make -C semantic-segmentation_amd/csrc` "
+                              "(or __graft_entry__.build()); there is no fallback path" % path)
+        spec = importlib.util.spec_from_file_location("_ddcn_tensors", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _tensors = module
+    return _tensors
 
 
 def check(rc):

@@ -103,3 +103,31 @@ def test_codes_are_unbiased_and_ordered():
 def test_another_seed_gives_other_numbers():
     a, b = ref.noise(np.arange(4096), 1), ref.noise(np.arange(4096), 2)
     assert (a[0] != b[0]).mean() > 0.99 and (a[1] != b[1]).mean() > 0.99
+
+
+def test_lists_of_tensors_are_described_and_marked():
+    t = _lib.tensors()
+    a, b, n = torch.zeros(6), torch.zeros(2, 3, dtype=torch.bfloat16), torch.zeros(0)
+    pointers, sizes, types, device, code, contiguous, distinct, given = t.describe([a, None, b, n, n])
+    assert list(array("Q", pointers)) == [a.data_ptr(), 0, b.data_ptr(), n.data_ptr(), n.data_ptr()]
+    assert list(array("q", sizes)) == [6, 0, 6, 0, 0] and list(array("i", types)) == [0, 0, 1, 0, 0]
+    assert (device, code, contiguous, distinct, given) == (-1, -2, True, True, 4)
+    assert t.describe([a.half(), a[:3].half()])[4] == 2 and t.describe([b.t()])[5] is False and t.describe([a, a])[6] is False
+    assert t.describe([a, a.double()])[4] == -1 and t.describe([a.double(), a])[4] == -1
+    assert t.describe([])[3:] == (-3, -3, True, True, 0) and t.describe([None])[3:] == (-3, -3, True, True, 0)
+    c = torch.zeros(2, 3, 4, 5).to(memory_format=torch.channels_last)
+    assert t.alike([a, b, c], [a, None, c.clone()]) == 0 and t.alike([c], [c.contiguous()]) == 1 and t.alike([b.t()], [b.t()]) == 1
+    assert t.alike([a], [a[:3]]) == 2 and t.alike([torch.zeros(7, 5, 1, 1).to(memory_format=torch.channels_last)], [torch.zeros(7, 5, 1, 1)]) == 0
+    versions = a._version, b._version
+    t.changed([a, b], [None, b])
+    t.changed([b])
+    assert (a._version, b._version) == (versions[0], versions[1] + 2)
+    with torch.inference_mode():
+        t.changed([torch.zeros(2)])
+    for bad in ((t.describe, (a,)), (t.describe, [3]), (t.describe, [torch.eye(3).to_sparse()]), (t.changed, (a,)), (t.alike, [a])):
+        with pytest.raises((TypeError, RuntimeError)):
+            bad[0](bad[1])
+    with pytest.raises(TypeError):
+        t.alike([a], [])
+    with pytest.raises(TypeError):
+        t.changed([a], [])
