@@ -361,7 +361,7 @@ typedef struct ddcn_adamw_hyper {
     int step;          /* t >= 1 of the bias corrections 1 - beta^t, for every tensor when `steps` is NULL */
     int dtype;         /* DDCN_F32 / DDCN_BF16 / DDCN_F16, of parameters and gradients */
     int bits;          /* of the moments: 32 or 8 */
-    unsigned seed;     /* of the random rounding of 8-bit codes */
+    unsigned seed;     /* of the random rounding of 8-bit codes: another one at every step */
 } ddcn_adamw_hyper;
 
 /* Elements of the moments' arena for `count` tensors: tensor i starts at the next multiple of 256 elements behind

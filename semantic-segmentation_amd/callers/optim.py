@@ -87,15 +87,17 @@ def _check_state(name, t, dtype, numel, device):
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
-               exp_avg_scale=None, exp_avg_sq_scale=None, seed=0, grad_norm=None, max_norm=None):
+               exp_avg_scale=None, exp_avg_sq_scale=None, seed=None, grad_norm=None, max_norm=None):
     """One AdamW step over `params` (list of tensors of one type: float32, bfloat16 or float16), in place.  They are
     contiguous or channels-last and do not overlap.
 
     `grads`: as many tensors of the same shapes, type and order in memory; None leaves a parameter and its moments as they
     are.  (Moments lie in the arena in the order of the parameter's memory.)
     `exp_avg`, `exp_avg_sq`: the arenas (`adamw_arena(params)` elements): float32, or int8 and uint8 with
-    `exp_avg_scale`, `exp_avg_sq_scale` (float32, one per 256 elements) and `seed`, a whole number that should differ
-    from step to step: it drives the unbiased rounding of the codes, and the same seed gives the same codes.
+    `exp_avg_scale`, `exp_avg_sq_scale` (float32, one per 256 elements) and `seed`, a whole number that has to differ
+    from step to step: it drives the random rounding of the codes, and the same seed gives the same codes.  None: the sum
+    of the step numbers.  (Under one seed again and again an element is rounded at one fixed threshold, and its moments
+    stand still where they should move.)
     `step`: t of the bias corrections, from 1 on, or one for each tensor.  With `max_norm` the gradients are scaled by
     min(1, max_norm / (grad_norm + 1e-6)), `grad_norm` being a float32 scalar on the GPU (see `grad_norm()`): nothing
     waits for it, and if it is not finite the step changes nothing.
@@ -149,6 +151,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
         steps, step = array("i", step), 1
         if len(steps) != len(params):
             raise RuntimeError("ddcn: %d parameters but %d step numbers" % (len(params), len(steps)))
+    if seed is None:
+        seed = step if steps is None else sum(steps)
     hyper = _lib.AdamwHyper(lr, betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, step,
                             code, bits, int(seed) & 0xFFFFFFFF)
     with _lib.on_device(dev):
@@ -271,8 +275,9 @@ class AdamW(torch.optim.Optimizer):
                 gs = [x if x is None or _same_order(x, p) else torch.empty_like(p).copy_(x) for p, x in zip(params, gs)]
             steps = [state[p]["step"] + (x is not None) for p, x in zip(params, gs)]
             same = steps[0] if steps.count(steps[0]) == len(steps) else None
-            # a seed for every step and arena; step numbers of one arena only grow
-            seed = self.seed + 0x10001 * number + 0x3779B1 * max(steps)
+            # a seed for every step and arena: the sum of an arena's step numbers grows at each of its steps (their maximum
+            # does not, where the gradients belong to tensors that have made fewer), and it comes back with a state dict
+            seed = self.seed + 0x10001 * number + 0x3779B1 * sum(steps)
             adamw_step(params, gs, arena.exp_avg, arena.exp_avg_sq, same or [max(s, 1) for s in steps], group["lr"],
                        group["betas"], group["eps"], group["weight_decay"], seed=seed, grad_norm=norm,
                        max_norm=self.max_norm, **arena.scales)

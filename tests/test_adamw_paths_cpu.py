@@ -1,0 +1,88 @@
+"""CPU: what `AdamW` hands to `adamw_step` over the life of a run, with the call itself replaced; states that are refused."""
+import importlib
+
+import numpy as np
+import pytest
+import torch
+
+import adamw_ref as ref
+from conftest import load_pkg
+
+load_pkg()
+callers = importlib.import_module("semantic-segmentation_amd.callers")
+optim = importlib.import_module("semantic-segmentation_amd.callers.optim")
+_lib = importlib.import_module("semantic-segmentation_amd.dcn._lib")
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The arguments of every adamw_step that an optimizer makes."""
+    seen = []
+    monkeypatch.setattr(optim, "adamw_step", lambda params, grads, m, v, step, lr, *a, **kw: seen.append(dict(kw, step=step, grads=grads, arena=m)))
+    return seen
+
+
+def _params(*sizes):
+    return [torch.nn.Parameter(torch.zeros(n)) for n in sizes]
+
+
+def _give(params, which):
+    for i, p in enumerate(params):
+        p.grad = torch.ones_like(p) if i in which else None
+
+
+def test_no_two_steps_of_an_arena_share_a_seed(calls):
+    """Whichever parameters have a gradient: staged training, branches taken at random, a new group."""
+    params = _params(3, 300, 5)
+    opt = callers.AdamW(params[:2], bits=8, seed=3)
+    turns = [{0}] * 4 + [{1}] * 6 + [{0, 1}, {1}, {0}, {0}, {1}]
+    for which in turns:
+        _give(params, which)
+        opt.step()
+    opt.add_param_group(dict(params=params[2:]))
+    for which in ({2}, {0, 2}, {1}, {2}):
+        _give(params, which)
+        opt.step()
+    arenas = {}
+    for c in calls:
+        arenas.setdefault(c["arena"].data_ptr(), []).append(c["seed"] & 0xFFFFFFFF)
+    assert [len(s) for s in arenas.values()] == [len(turns) + 2, 3]
+    assert all(len(set(s)) == len(s) for s in arenas.values())
+
+
+def test_seeds_go_on_behind_a_state_dict(calls):
+    params = _params(3, 300)
+    opt = callers.AdamW(params, bits=8, seed=3)
+    for which in ({0}, {0}, {1}):
+        _give(params, which)
+        opt.step()
+    again = callers.AdamW(params, bits=8, seed=3)
+    again.load_state_dict(opt.state_dict())
+    for o in (opt, again):
+        _give(params, {1})
+        o.step()
+    assert calls[-1]["seed"] == calls[-2]["seed"] and len({c["seed"] for c in calls}) == 4
+
+
+def test_a_seed_that_repeats_makes_moments_stand_still():
+    """Why it matters, from the formulas: second moments of gradients that drop by ten, 1500 steps (beta2 0.999: the mean root
+    falls to 0.481); with one seed at every step the rounding is a threshold, and they stop where it says so."""
+    def root(seed_of):
+        n, b2 = 256, 0.999
+        g = np.ones(n, np.float32)
+        r = g.copy()
+        g[128:] = 0.1
+        for t in range(1500):
+            r = np.sqrt(ref.moments32(g, g * 0, (r * r).astype(np.float32), 0.9, b2)[1]).astype(np.float32)
+            q, s = ref.encode(r, ref.noise(np.arange(n), seed_of(t))[1], 255)
+            r = ref.decode_r(np.maximum(q, 1), s)
+        return r[128:].mean()
+
+    want = np.sqrt(0.999 ** 1500 + (1 - 0.999 ** 1500) * 0.01)
+    assert abs(root(lambda t: t) / want - 1) < 0.25          # as derived in the GPU test of the same experiment
+    assert root(lambda t: 7) > 0.9
+
+
+def test_a_step_without_a_seed_takes_one_from_its_step_number():
+    import inspect
+    assert inspect.signature(callers.adamw_step).parameters["seed"].default is None
