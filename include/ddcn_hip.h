@@ -374,8 +374,8 @@ long long ddcn_adamw_arena(int count, const long long *numels);
  * 256 elements in `exp_avg_scale` / `exp_avg_sq_scale`).  `grad_norm`: one fp32 on the device, or NULL for no clipping;
  * a norm that is not finite leaves everything as it was.  The arithmetic (fl = one rounding to fp32):
  *   g' = fl(c g), c = fl(min(1, max_norm / (norm + 1e-6)));  m = fl(b1 m + (1-b1) g');  v = fl(b2 v + ((1-b2) g') g');
- *   r = fl(sqrt(v));  p <- p (1 - lr wd) - lr / (1 - b1^t) m / (r / sqrt(1 - b2^t) + eps), in fp32, rounded once to the
- *   parameter's type.
+ *   r = fl(sqrt(v));  p <- p (1 - lr wd) - lr / (1 - b1^t) m / (r / sqrt(1 - b2^t) + eps), in fp32 (1 - lr wd in
+ *   two parts, so that a decay below half a step of fp32 still joins the update), rounded once to the parameter's type.
  * A signed code q stands for m = s q|q|, s = max|m| / 127^2 of its 256 elements; an unsigned one for r = s q^2,
  * s = max r / 255^2.  |q| = floor(sqrt(x / s) + u) with u in [0, 1) hashed from (seed, place in the arena): unbiased, so
  * that a moment moves by less than a code per step on average (to nearest, it would stand still); r > 0 keeps q >= 1, so

@@ -102,7 +102,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
     min(1, max_norm / (grad_norm + 1e-6)), `grad_norm` being a float32 scalar on the GPU (see `grad_norm()`): nothing
     waits for it, and if it is not finite the step changes nothing.
 
-    Everything else is as in torch.optim.AdamW: p <- p (1 - lr wd) - lr m^ / (sqrt(v^) + eps).  The step number, lr and
+    Everything else is as in torch.optim.AdamW: p <- p (1 - lr wd) - lr m^ / (sqrt(v^) + eps), decay and update rounded
+    together to the parameter's type (a 16-bit parameter does not see changes below half its step).  The step number, lr and
     seed are fixed when the call is made, so it refuses to be captured into a HIP graph."""
     params, grads = list(params), list(grads)
     if len(params) != len(grads):

@@ -31,7 +31,8 @@ struct AdamwArgs {
     const float *norm;
     long long first;       // block of the arena that the launch begins with
     unsigned blocks;       // of the launch
-    float b1, ob1, b2, ob2, eps, decay, max_norm;
+    float b1, ob1, b2, ob2, eps, max_norm;
+    float decay, decay_rest;   // their sum is 1 - lr wd, to 48 bits
     float step_size;       // lr / (1 - beta1^t)
     float rsqrt_bc2;       // 1 / sqrt(1 - beta2^t)
     unsigned seed;
@@ -185,6 +186,7 @@ __device__ __forceinline__ void update_block(const AdamwArgs &a, const Place &w,
     }
     // The parameter's own arithmetic may be fused and take the hardware's roots: nothing is decided on its last bits.
     // Without an eps that hides it, a root of the smallest numbers has to be right.
+    // Small decays (lr wd below 2^-25 makes 1 - lr wd one in fp32) join the update before the one rounding at p.
     if (a.eps >= 0x1p-40f) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = __builtin_amdgcn_sqrtf(v[e]);
@@ -194,7 +196,7 @@ __device__ __forceinline__ void update_block(const AdamwArgs &a, const Place &w,
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        h.p[e] = fmaf(-a.step_size, m[e] * __builtin_amdgcn_rcpf(fmaf(r[e], a.rsqrt_bc2, a.eps)), h.p[e] * a.decay);
+        h.p[e] = fmaf(h.p[e], a.decay, fmaf(-a.step_size, m[e] * __builtin_amdgcn_rcpf(fmaf(r[e], a.rsqrt_bc2, a.eps)), h.p[e] * a.decay_rest));
     if (wide) store_four<DT>(w.p, w.i, h.p);
     else store_some<DT>(w.p, w.i, w.live, false, h.p);
     if (BITS == 32) {
@@ -465,7 +467,11 @@ int ddcn_adamw_step(int count, const unsigned long long *params, const unsigned 
     a.b2 = (float)h->beta2;
     a.ob2 = (float)(1.0 - h->beta2);
     a.eps = (float)h->eps;
-    a.decay = (float)(1.0 - h->lr * h->weight_decay);
+    // 1 - lr wd towards zero, and the rest, of the same sign and never zero beside it: an infinite p stays infinite
+    const double decay = 1.0 - h->lr * h->weight_decay;
+    a.decay = (float)decay;
+    if (fabs((double)a.decay) > fabs(decay)) a.decay = nextafterf(a.decay, 0.f);
+    a.decay_rest = a.decay == 0.f ? 0.f : (float)copysign(fmax(fabs(decay - a.decay), 0x1p-100), decay);
     a.max_norm = grad_norm ? (float)h->max_norm : 0.f;
     a.seed = h->seed;
     a.count = 0;

@@ -58,3 +58,41 @@ def test_steps_without_a_seed_round_differently():
         return m
     assert torch.equal(codes(5), codes(5, seed=5)) and torch.equal(codes([5, 9]), codes([5, 9], seed=14))
     assert not torch.equal(codes(5), codes(6))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_weight_decay_below_half_a_step_of_float32(bits):
+    """lr wd = 2.5e-8 (lr 2.5e-4, weight decay 1e-4): 1 - lr wd is 1 in float32, but parameters that move anyway are decayed.
+    p in [1, 2), gradients of random signs.  After k steps the mean of p, less what p would be without decay (float64 from the
+    moments of a float32 run, or from the decoded ones), is -k lr wd mean(p) = -1.5e-5.  Off by: the rounding of p, 2^-23 /
+    sqrt(12) a step and element, its mean over n = 2^16 elements and k = 400 steps 2.7e-9; and the float32 arithmetic of the
+    update, 16 half steps of 2^-24 of lr max|m^ / sqrt(v^)| (3 at most here) a step, 2.9e-7 if they all had one sign."""
+    n, k, lr, wd = 1 << 16, 400, 2.5e-4, 1e-4
+    b1, b2 = BETAS
+    g = _rng(5)
+    p = (1 + torch.rand(n, generator=g)).to(DEV)
+    want = p.double()
+    m, v = (torch.zeros(n, device=DEV, dtype=t) for t in ((torch.float32,) * 2 if bits == 32 else (torch.int8, torch.uint8)))
+    scales = [] if bits == 32 else [torch.zeros(n // 256, device=DEV) for _ in range(2)]
+    for t in range(1, k + 1):
+        grad = torch.randn(n, generator=g).to(DEV)
+        om, ov = (m, v) if bits == 32 else callers.adamw_moments(m, v, *scales)
+        om, ov = om.double() * b1 + (1 - b1) * grad.double(), ov.double() * b2 + (1 - b2) * grad.double() ** 2
+        update = om / (1 - b1 ** t) / ((ov / (1 - b2 ** t)).sqrt() + EPS)
+        assert float(update.abs().max()) < (3 if bits == 32 else 10)
+        want = want * (1 - lr * wd) - lr * update
+        callers.adamw_step([p], [grad], m, v, t, lr, BETAS, EPS, wd, *scales, **({} if bits == 32 else dict(seed=t)))
+    drift, off = k * lr * wd * 1.5, float((p.double() - want).mean())
+    assert drift > 1.4e-5 and abs(off) < (3e-7 if bits == 32 else 1e-6), off
+
+
+def test_step_of_parameters_that_are_not_finite_or_at_the_end_of_the_range():
+    """The decay leaves an infinity what it is, with and without weight decay; so does a NaN stay one, alone."""
+    top = torch.finfo(torch.float32).max
+    p0 = torch.tensor([float("inf"), -float("inf"), float("nan"), top, -top, 0.0, 1e-40, 3.0], device=DEV)
+    for lr, wd in ((1e-3, 0.0), (2.5e-4, 1e-4), (1e-2, 0.05), (1.0, 1.0), (1.0, 1.5), (0.0, 0.1)):
+        p = p0.clone()
+        callers.adamw_step([p], [torch.zeros(8, device=DEV)], torch.zeros(256, device=DEV), torch.zeros(256, device=DEV), 1, lr, BETAS, EPS, wd)
+        d = 1 - lr * wd
+        want = (p0.double() * d).float()             # (inf * 0 is NaN)
+        assert torch.equal(torch.isnan(p), torch.isnan(want)) and torch.equal(p.nan_to_num(7.0), want.nan_to_num(7.0)), (lr, wd, p)
