@@ -7,6 +7,8 @@ over the layers around them: a bottleneck's 1x1 convolutions, the depth branch, 
 A token that holds a NaN or an infinity gives NaN in all of its outputs.  Kernels: csrc/ddcn_int8.hip; the arithmetic is
 written down in include/ddcn_hip.h.  CPU tensors raise NotImplementedError, tensors that require grad a RuntimeError.
 """
+import math
+
 import torch
 import torch.nn as nn
 
@@ -37,7 +39,13 @@ def _check_same_device(name, t, dev, x):
         raise RuntimeError("ddcn: %s is on %s but the input is on %s" % (name, t.device, x.device))
 
 
-def _check_weight(x, dev, weight_q, weight_scale, bias, k):
+def _check_sizes(tokens, k, n=0):
+    """Before they become 32-bit fields of a struct, which keep the low bits of what does not fit."""
+    if (tokens | k | n) >> 31:
+        raise RuntimeError("ddcn: %d tokens of %d values, %d channels: 2^31 and more are not supported" % (tokens, k, n))
+
+
+def _check_weight(x, dev, weight_q, weight_scale, bias, tokens, k):
     """-> (channels, weights with contiguous values in a row, the rows' stride in bytes, scales, float32 bias)"""
     _check_same_device("weight_q", weight_q, dev, x)
     _check_same_device("weight_scale", weight_scale, dev, x)
@@ -45,6 +53,7 @@ def _check_weight(x, dev, weight_q, weight_scale, bias, k):
     if weight_q.dtype is not _INT8 or len(shape) != 2 or shape[1] != k:
         raise RuntimeError("ddcn: weight_q has to be int8 [channels, %d], got %s %s" % (k, weight_q.dtype, tuple(shape)))
     n = shape[0]
+    _check_sizes(tokens, k, n)
     if weight_scale.dtype is not _F32 or weight_scale.shape != (n,):
         raise RuntimeError("ddcn: weight_scale has to be float32 [%d], got %s %s" % (n, weight_scale.dtype, tuple(weight_scale.shape)))
     if bias is not None:
@@ -89,6 +98,7 @@ def quantize_int8(x):
     if x.dim() != 2:
         raise RuntimeError("ddcn: 2D tensor expected but got: %d" % x.dim())
     rows, k = x.shape
+    _check_sizes(rows, k)
     if k > 1 and x.stride(1) != 1:
         x = x.contiguous()
     q = torch.empty((rows, k), dtype=torch.int8, device=x.device)
@@ -109,7 +119,8 @@ def int8_linear(input, weight_q, weight_scale, bias=None, relu=False, out_dtype=
     if not shape:
         raise RuntimeError("ddcn: input has no dimension")
     k, dev = shape[-1], input.get_device()
-    n, weight_q, ldw, weight_scale, bias = _check_weight(input, dev, weight_q, weight_scale, bias, k)
+    tokens = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    n, weight_q, ldw, weight_scale, bias = _check_weight(input, dev, weight_q, weight_scale, bias, tokens, k)
     dtype = input.dtype if out_dtype is None else out_dtype
     out = _out_type(dtype)
     y = torch.empty(shape[:-1] + (n,), dtype=dtype, device=input.device)
@@ -134,10 +145,10 @@ def int8_conv1x1(input, weight_q, weight_scale, bias=None, stride=1, relu=False,
     stride = int(stride)
     images, c, h, w = input.shape
     dev = input.get_device()
-    n, weight_q, ldw, weight_scale, bias = _check_weight(input, dev, weight_q, weight_scale, bias, c)
+    ho, wo = -(-h // stride), -(-w // stride)
+    n, weight_q, ldw, weight_scale, bias = _check_weight(input, dev, weight_q, weight_scale, bias, images * ho * wo, c)
     dtype = input.dtype if out_dtype is None else out_dtype
     out = _out_type(dtype)
-    ho, wo = -(-h // stride), -(-w // stride)
     si, sk, sh, sw = input.stride()
     last = c > 1 and sk == 1
     y = torch.empty((images, n, ho, wo), dtype=dtype, device=input.device,
