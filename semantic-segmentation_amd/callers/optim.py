@@ -275,11 +275,12 @@ class AdamW(torch.optim.Optimizer):
             if _lib.tensors().alike(params, gs) == 1:
                 gs = [x if x is None or _same_order(x, p) else torch.empty_like(p).copy_(x) for p, x in zip(params, gs)]
             steps = [state[p]["step"] + (x is not None) for p, x in zip(params, gs)]
-            same = steps[0] if steps.count(steps[0]) == len(steps) else None
+            live = {s for s, x in zip(steps, gs) if x is not None}       # the others' numbers do not count
             # a seed for every step and arena: the sum of an arena's step numbers grows at each of its steps (their maximum
             # does not, where the gradients belong to tensors that have made fewer), and it comes back with a state dict
             seed = self.seed + 0x10001 * number + 0x3779B1 * sum(steps)
-            adamw_step(params, gs, arena.exp_avg, arena.exp_avg_sq, same or [max(s, 1) for s in steps], group["lr"],
+            adamw_step(params, gs, arena.exp_avg, arena.exp_avg_sq,
+                       live.pop() if len(live) == 1 else [max(s, 1) for s in steps], group["lr"],
                        group["betas"], group["eps"], group["weight_decay"], seed=seed, grad_norm=norm,
                        max_norm=self.max_norm, **arena.scales)
             for p, s in zip(params, steps):

@@ -21,7 +21,7 @@ constexpr long long kMaxGrid = 1LL << 23;   // workgroups of a launch: 256 threa
 constexpr int kMaxTensors = 160;
 struct AdamwArgs {
     // tensor j of the launch covers the arena's blocks block0[j] .. block0[j+1]-1 (relative to `first`); n[j] elements.
-    // A null gradient: its blocks are left alone.
+    // A null gradient: blocks between the tensors that are left alone.
     void *p[kMaxTensors];
     const void *g[kMaxTensors];
     unsigned block0[kMaxTensors];
@@ -405,6 +405,10 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 // 8 bits: two, whose loads then hide behind the other's arithmetic (107 us; 123 with one, 110 with four) -- but one where
 // two would leave CUs without work.
 constexpr unsigned kSpreadBlocks = 8192;
+// Blocks of tensors without a gradient that a launch may hold between two others, as one entry whose waves end at once: below,
+// they cost less than a launch more (two tensors of 16 blocks, fp32: 4.5 us in two launches; in one 2.6 with 1024 blocks
+// between them, 3.6 with 8192, 4.8 with 16384, 42 with 262144; with 8-bit moments 6.1, and 3.4, 5.7, 7.0, 48).
+constexpr long long kMaxGap = 8192;
 template <int DT, int BITS> void launch_adamw(const AdamwArgs &a, hipStream_t s)
 {
     constexpr int kMany = BITS == 32 ? 1 : 2;
@@ -478,12 +482,10 @@ int ddcn_adamw_step(int count, const unsigned long long *params, const unsigned 
     a.blocks = 0;
     a.first = 0;
     a.step_size = a.rsqrt_bc2 = 0.f;
-    long long block = 0;
+    long long block = 0;       // of the arena, where the next tensor starts
     int known = 0;
-    bool any = false;          // a gradient among the launch's tensors
     auto launch = [&]() -> int {
-        const bool due = any;
-        any = false;
+        const bool due = a.count > 0;
         if (due) {
             hipStream_t s = (hipStream_t)stream;
             if (h->dtype == DDCN_F32) h->bits == 32 ? launch_adamw<DDCN_F32, 32>(a, s) : launch_adamw<DDCN_F32, 8>(a, s);
@@ -492,10 +494,13 @@ int ddcn_adamw_step(int count, const unsigned long long *params, const unsigned 
         }
         a.count = 0;
         a.blocks = 0;
-        a.first = block;
         return due ? check_launch("adamw") : DDCN_OK;
     };
     for (int i = 0; i < count; ++i) {
+        if (!grads[i] || !numels[i]) {        // no gradient: its step number does not matter either
+            block += ceil_div(numels[i], kBlock);
+            continue;
+        }
         const int step = steps ? steps[i] : h->step;
         if (step != known) {       // one step number to a launch
             const int rc = launch();
@@ -507,17 +512,26 @@ int ddcn_adamw_step(int count, const unsigned long long *params, const unsigned 
         // a tensor of 2^31 elements and more goes in pieces
         for (long long done = 0; done < numels[i]; done += 1LL << 31) {
             const long long n = numels[i] - done < (1LL << 31) ? numels[i] - done : 1LL << 31, blocks = ceil_div(n, kBlock);
-            if (a.count == kMaxTensors || a.blocks + blocks > kMaxGrid * kWaves) {
+            // blocks of the arena since the launch's last tensor, of tensors without a gradient
+            const long long gap = a.count ? block - (a.first + a.blocks) : 0;
+            if (gap > kMaxGap || a.count + (gap > 0) >= kMaxTensors || a.blocks + gap + blocks > kMaxGrid * kWaves) {
                 const int rc = launch();
                 if (rc != DDCN_OK) return rc;
             }
+            if (!a.count) a.first = block;
+            else if (gap) {
+                a.p[a.count] = nullptr;
+                a.g[a.count] = nullptr;
+                a.block0[a.count] = a.blocks;
+                a.n[a.count++] = 0;
+                a.blocks += (unsigned)gap;
+            }
             a.p[a.count] = (void *)(params[i] + done * size);
-            a.g[a.count] = grads[i] ? (const void *)(grads[i] + done * size) : nullptr;
+            a.g[a.count] = (const void *)(grads[i] + done * size);
             a.block0[a.count] = a.blocks;
             a.n[a.count++] = (unsigned)n;
             a.blocks += (unsigned)blocks;
             block += blocks;
-            any = any || grads[i];
         }
     }
     return launch();

@@ -86,3 +86,14 @@ def test_a_seed_that_repeats_makes_moments_stand_still():
 def test_a_step_without_a_seed_takes_one_from_its_step_number():
     import inspect
     assert inspect.signature(callers.adamw_step).parameters["seed"].default is None
+
+
+def test_step_numbers_of_parameters_without_a_gradient_do_not_count(calls):
+    """One number for the call where all that move share one, whatever the frozen ones' are."""
+    params = _params(3, 300, 5)
+    opt = callers.AdamW(params)
+    for which in ({0, 1, 2}, {0, 2}, {0, 2}, {1, 2}):
+        _give(params, which)
+        opt.step()
+    assert [c["step"] for c in calls] == [1, 2, 3, [3, 2, 4]]
+    assert [opt.state[p]["step"] for p in params] == [3, 2, 4]

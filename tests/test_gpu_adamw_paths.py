@@ -96,3 +96,71 @@ def test_step_of_parameters_that_are_not_finite_or_at_the_end_of_the_range():
         d = 1 - lr * wd
         want = (p0.double() * d).float()             # (inf * 0 is NaN)
         assert torch.equal(torch.isnan(p), torch.isnan(want)) and torch.equal(p.nan_to_num(7.0), want.nan_to_num(7.0)), (lr, wd, p)
+
+
+def _launches(params, grads, steps):
+    """Kernel nodes of one C call over float32 tensors (captured, not run)."""
+    import ctypes
+    from array import array
+    numels = [p.numel() for p in params]
+    n = callers.adamw_arena(params)
+    m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    lists = [array("Q", [p.data_ptr() for p in params]), array("Q", [0 if g is None else g.data_ptr() for g in grads]),
+             array("q", numels), array("i", steps)]
+    hyper = _lib.AdamwHyper(LR, *BETAS, EPS, WD, 0.0, 1, 0, 32, 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        rc = _lib.lib().ddcn_adamw_step(len(params), *(ctypes.c_void_p(a.buffer_info()[0]) for a in lists), _lib.ptr(m), _lib.ptr(v),
+                                        None, None, None, hyper, _lib.stream_of(0))
+    assert rc == 0
+    count = ctypes.c_size_t(0)
+    assert _lib.lib().hipGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(count)) == 0
+    return count.value
+
+
+def test_tensors_without_a_gradient_do_not_split_launches():
+    """Convolutions between frozen norm layers: their step numbers stay behind, and no launch needs them."""
+    sizes = [4096, 64, 64] * 53
+    params = [torch.zeros(n, device=DEV) for n in sizes]
+    grads = [torch.zeros(n, device=DEV) if i % 3 == 0 else None for i, n in enumerate(sizes)]
+    assert _launches(params, grads, [9 if g is not None else 1 for g in grads]) == 1
+    assert _launches(params, [torch.zeros_like(p) for p in params], [9] * 159) == 1
+    # two step numbers among those that count: a launch where they change
+    assert _launches(params[:9], grads[:9], [3, 1, 1, 3, 2, 7, 5, 1, 1]) == 2
+    # more blocks in between than a launch is worth
+    far = torch.zeros(8193 * 256, device=DEV)
+    for n, launches in ((8192, 1), (8193, 2)):
+        assert _launches([params[0], far[:n * 256], params[3]], [grads[0], None, grads[3]], [9, 1, 9]) == launches
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_frozen_parameters_between_others_over_steps(bits):
+    """Gradients that come and go (None in turn, stale step numbers): every parameter as if it were alone in its own call."""
+    sizes = [300, 7, 256, 5000, 64, 64, 2049, 1, 513] * 3
+    g = _rng(8)
+    start = [torch.randn(n, generator=g).to(DEV) for n in sizes]
+    together, alone = [p.clone() for p in start], [p.clone() for p in start]
+    types = (torch.float32,) * 2 if bits == 32 else (torch.int8, torch.uint8)
+    new = lambda n: [torch.zeros(n, dtype=t, device=DEV) for t in types] + [torch.zeros(n // 256, device=DEV) for _ in range(2)][:0 if bits == 32 else 2]   # noqa: E731
+    state, each = new(callers.adamw_arena(start)), [new(callers.adamw_arena([p])) for p in start]
+    at = ref.starts_of(sizes)[0]
+    steps = [0] * len(sizes)
+    for t in range(5):
+        grads = [None if i % 3 == 1 or (i + t) % 4 == 0 or (i > 20 and t > 2) else torch.randn(n, generator=g).to(DEV) for i, n in enumerate(sizes)]
+        steps = [s + (x is not None) for s, x in zip(steps, grads)]
+        seeds = {} if bits == 32 else dict(seed=t)
+        before = [[x.clone() for x in s] for s in each]
+        callers.adamw_step(together, grads, state[0], state[1], [max(s, 1) for s in steps], LR, BETAS, EPS, WD, *state[2:], **seeds)
+        for i, (p, x, s, b) in enumerate(zip(alone, grads, each, before)):
+            if x is not None:          # from the moments that the common call found: codes depend on a tensor's place
+                callers.adamw_step([p], [x], s[0], s[1], steps[i], LR, BETAS, EPS, WD, *s[2:], **seeds)
+            assert torch.equal(together[i], p), (t, i)
+            n = -(-sizes[i] // 256) * 256
+            now = [state[0][at[i]:at[i] + n], state[1][at[i]:at[i] + n]] + [q[at[i] // 256:(at[i] + n) // 256] for q in state[2:]]
+            if bits == 32 or x is None:
+                assert all(torch.equal(c, d) for c, d in zip(now, s)), (t, i)
+            else:                      # (the scales do not)
+                assert all(torch.equal(c, d) for c, d in zip(now[2:], s[2:])), (t, i)
+                for c, d in zip(now, s):
+                    d.copy_(c)
