@@ -55,14 +55,16 @@ def adamw_arena(params):
 
 def grad_norm(grads):
     """sqrt of the sum of squares over all `grads` (entries may be None), a float32 scalar on their GPU: summed in
-    float64 in a fixed order, so that it is the same at every call.  Types may be mixed."""
+    float64 in a fixed order, so that it is the same at every call.  Types may be mixed.  Any strides: a gradient that is
+    neither contiguous nor channels-last is copied first.  Not differentiable."""
     grads = [g for g in grads if g is not None]
     if not grads:
         raise RuntimeError("ddcn: grad_norm needs at least one gradient")
     pointers, numels, dtypes, dev, dtype, contiguous, _, _ = _lib.tensors().describe(grads)
     _check_device(dev, "gradients")
     if not contiguous and not all(map(_dense, grads)):
-        raise RuntimeError("ddcn: gradient tensors have to be contiguous (or channels-last)")
+        grads = [g if _dense(g) else g.detach().contiguous() for g in grads]
+        pointers = _lib.tensors().describe(grads)[0]
     if dtype == -1:
         other = next(g.dtype for g in grads if g.dtype not in _lib.ELEMENT_TYPES)
         raise RuntimeError("ddcn: %s gradients are not supported (float32, float16, bfloat16)" % other)

@@ -164,3 +164,38 @@ def test_frozen_parameters_between_others_over_steps(bits):
                 assert all(torch.equal(c, d) for c, d in zip(now[2:], s[2:])), (t, i)
                 for c, d in zip(now, s):
                     d.copy_(c)
+
+
+def test_gradients_of_any_strides_are_measured_and_clipped():
+    """What the optimizer takes without max_norm it takes with it: transposed and expanded gradients."""
+    g = _rng(12)
+    w, x = torch.randn(40, 30, generator=g).to(DEV), torch.randn(30, 40, generator=g).to(DEV).t()
+    e = torch.full((1, 1), 0.25, device=DEV).expand(40, 30)
+    part = torch.randn(40, 60, generator=g).to(DEV)[:, ::2]
+    for grad in (x, e, part):
+        assert not grad.is_contiguous()
+        norm = callers.grad_norm([grad, None, w])
+        assert float(norm) == float(callers.grad_norm([grad.contiguous(), w]))
+        exact = np.sqrt((_np(grad).astype(np.float64) ** 2).sum() + (_np(w).astype(np.float64) ** 2).sum())
+        assert abs(float(norm) - exact) <= 2.0 ** -24 * exact * (1 + 1e-6)
+        params = [torch.nn.Parameter(w.clone()) for _ in range(2)]
+        for p, y in zip(params, (grad, grad.contiguous())):
+            opt = callers.AdamW([p], lr=LR, max_norm=0.5)
+            p.grad = y
+            opt.step()
+        assert torch.equal(*params) and not torch.equal(params[0], w)
+
+
+def test_norm_of_strided_gradients_in_a_graph():
+    x = torch.randn(300, 200, generator=_rng(13)).to(DEV)
+    callers.grad_norm([x.t()])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = callers.grad_norm([x.t(), x])
+    for k in range(3):
+        x.mul_(1.5 + k)
+        eager = float(callers.grad_norm([x.t(), x]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert float(out) == eager
