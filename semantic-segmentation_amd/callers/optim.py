@@ -289,19 +289,33 @@ class AdamW(torch.optim.Optimizer):
                 state[p]["step"] = s
         return loss
 
+    def _check_saved(self, p, saved):
+        """Refuses a parameter's saved state that `_take` could not copy."""
+        want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.bits == 8 else set())
+        found = "%s" % {k: getattr(t, "dtype", t) for k, t in saved.items()}
+        if set(saved) != want or not all(torch.is_tensor(t) for k, t in saved.items() if k != "step"):
+            raise ValueError("the state dict holds %s, not the state of AdamW with bits=%d" % (found, self.bits))
+        moments = saved["exp_avg"], saved["exp_avg_sq"]
+        scales = [saved[k] for k in sorted(want) if k.endswith("scale")]
+        types = all(t.is_floating_point() for t in moments) if self.bits == 32 else \
+            [t.dtype for t in moments] == [torch.int8, torch.uint8]
+        if not types or any(t.shape != p.shape for t in moments) or any(t.shape != (-(-p.numel() // BLOCK),) for t in scales):
+            raise ValueError("the state dict holds %s, not the state of AdamW with bits=%d over these parameters"
+                             % (found, self.bits))
+        if self.bits == 8 and not all(_same_order(t, p) for t in moments):      # codes and their scales go by memory
+            raise ValueError("8-bit moments of a parameter in another memory format")
+        if int(saved["step"]) < 0:
+            raise ValueError("step number %r" % (saved["step"],))
+
     def load_state_dict(self, state_dict):
         """As torch's, but moments keep their types (torch would cast them to the parameter's) and are copied into the
-        arenas.  A state of another number of bits is refused."""
+        arenas.  A state of another number of bits, or over other parameters, is refused and changes nothing."""
         saved, order = state_dict["state"], {}
         for group, old in zip(self.param_groups, state_dict["param_groups"]):
             order.update(zip(group["params"], old["params"]))
         loaded = {p: saved[i] for p, i in order.items() if i in saved}
-        want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.bits == 8 else set())
         for p, theirs in loaded.items():
-            if set(theirs) != want or (theirs["exp_avg"].dtype == torch.int8) != (self.bits == 8) or \
-                    theirs["exp_avg"].shape != p.shape:
-                raise ValueError("the state dict holds %s, not the state of AdamW with bits=%d over these parameters"
-                                 % ({k: getattr(t, "dtype", t) for k, t in theirs.items()}, self.bits))
+            self._check_saved(p, theirs)
         super().load_state_dict(dict(state_dict, state={}))
         self._take(loaded)
 
@@ -315,14 +329,12 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 self._arena(g, dtype, params)
                 for p in params:
+                    mine = self.state[p]
                     for k, t in loaded.get(p, {}).items():
-                        mine = self.state[p]
                         if k == "step":
                             mine[k] = int(t)
-                            continue
-                        if self.bits == 8 and not _same_order(t, mine[k]):      # codes and their scales go by memory
-                            raise ValueError("8-bit moments of a parameter in another memory format")
-                        mine[k].copy_(t)
+                        else:
+                            mine[k].copy_(t)
 
     def __getstate__(self):          # copy.deepcopy and pickle: torch's own leaves a subclass's attributes out
         return dict(super().__getstate__(), settings=(self.bits, self.max_norm, self.seed))

@@ -97,3 +97,56 @@ def test_step_numbers_of_parameters_without_a_gradient_do_not_count(calls):
         opt.step()
     assert [c["step"] for c in calls] == [1, 2, 3, [3, 2, 4]]
     assert [opt.state[p]["step"] for p in params] == [3, 2, 4]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_dict_that_is_refused_changes_nothing(calls, bits):
+    """Whatever is wrong with it, and at whichever parameter: moments, step numbers and settings stay, and steps go on."""
+    make = lambda: [torch.nn.Parameter(torch.randn(5, 6, 3, 3)), torch.nn.Parameter(torch.zeros(300))]     # noqa: E731
+    params, others = make(), make()
+    others[1].data = others[1].data[:300]
+    opt, theirs = callers.AdamW(params, bits=bits, lr=0.5), callers.AdamW(others, bits=bits, lr=0.25)
+    for o, ps in ((opt, params), (theirs, others)):
+        for _ in range(3):
+            _give(ps, {0, 1})
+            o.step()
+    for p in params:
+        opt.state[p]["exp_avg"].fill_(3)
+    good = theirs.state_dict()
+
+    def with_(index, name, value):
+        state = {i: dict(s) for i, s in good["state"].items()}
+        if value is None:
+            del state[index][name]
+        else:
+            state[index][name] = value
+        return dict(good, state=state)
+
+    last = good["state"][0]["exp_avg"].to(memory_format=torch.channels_last)
+    bad = [with_(1, "exp_avg_sq", good["state"][1]["exp_avg_sq"][:1]), with_(1, "exp_avg", good["state"][1]["exp_avg"][:299]),
+           with_(1, "exp_avg_sq", None), with_(1, "max_exp_avg_sq", torch.zeros(300)), with_(1, "step", None),
+           with_(1, "step", "three"), with_(1, "step", -1), with_(1, "exp_avg", 4.0),
+           dict(good, param_groups=good["param_groups"] * 2), dict(good, param_groups=[dict(good["param_groups"][0], params=[0])])]
+    if bits == 8:
+        bad += [with_(0, "exp_avg", last), with_(1, "exp_avg_scale", good["state"][1]["exp_avg_scale"][:1]),
+                with_(1, "exp_avg_sq", good["state"][1]["exp_avg_sq"].float())]
+    before = [(id(opt.state[p]["exp_avg"]), opt.state[p]["exp_avg"].clone(), opt.state[p]["step"]) for p in params]
+    for state_dict in bad:
+        with pytest.raises((ValueError, TypeError)):
+            opt.load_state_dict(state_dict)
+        for p, (name, m, step) in zip(params, before):
+            assert id(opt.state[p]["exp_avg"]) == name and torch.equal(opt.state[p]["exp_avg"], m) and opt.state[p]["step"] == step
+        assert opt.param_groups[0]["lr"] == 0.5
+    _give(params, {0, 1})
+    opt.step()
+    assert calls[-1]["step"] == 4
+    opt.load_state_dict(good)
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.state[params[1]]["step"] == 3 and not opt.state[params[1]]["exp_avg"].any()
+    if bits == 32:              # torch.optim.AdamW's own state: a step number in a tensor, any memory format, any type
+        opt.load_state_dict(with_(0, "exp_avg", last.double() + 2))
+        assert (opt.state[params[0]]["exp_avg"] == 2).all()
+    opt.load_state_dict(with_(0, "step", torch.tensor(7.0)))
+    assert opt.state[params[0]]["step"] == 7
+    empty = callers.AdamW(make(), bits=bits).state_dict()
+    opt.load_state_dict(empty)
+    assert not opt.state
