@@ -11,6 +11,7 @@ import math
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -26,10 +27,16 @@ def _element_type(name, t):
     code = _lib.ELEMENT_TYPES.get(t.dtype)
     if code is None:
         raise RuntimeError("ddcn: %s of %s is not supported (float32, float16, bfloat16)" % (name, t.dtype))
-    if t.requires_grad and torch.is_grad_enabled():
+    _check_no_gradient(name, t)
+    return code
+
+
+def _check_no_gradient(name, t):
+    """Neither a backward pass through t is asked for nor does it carry a forward-mode tangent (which no_grad does not stop)."""
+    if t.requires_grad and torch.is_grad_enabled() or \
+            forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         raise RuntimeError("ddcn: the 8-bit layers have no backward pass: call them under torch.no_grad(), or detach %s"
                            % name)
-    return code
 
 
 def _check_same_device(name, t, dev, x):
@@ -56,6 +63,7 @@ def _check_weight(x, dev, weight_q, weight_scale, bias, tokens, k):
     _check_sizes(tokens, k, n)
     if weight_scale.dtype is not _F32 or weight_scale.shape != (n,):
         raise RuntimeError("ddcn: weight_scale has to be float32 [%d], got %s %s" % (n, weight_scale.dtype, tuple(weight_scale.shape)))
+    _check_no_gradient("weight_scale", weight_scale)
     if bias is not None:
         _check_same_device("bias", bias, dev, x)
         if bias.dtype not in _lib.ELEMENT_TYPES or bias.shape != (n,):

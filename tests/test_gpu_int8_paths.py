@@ -51,3 +51,28 @@ def test_sizes_that_32_bits_do_not_hold_are_refused():
     assert torch.cuda.max_memory_allocated() == before
     y = pkg.int8_conv1x1(row.view(1, 8, 1, 1).expand(1, 8, far, 1), wq, ws, b, stride=far)       # one pixel of it
     assert torch.equal(y.view(6), pkg.int8_linear(row, wq, ws, b).view(6))
+
+
+def test_gradients_asked_for_are_refused_not_dropped():
+    """There is no backward pass: whatever requires a gradient, and forward-mode tangents."""
+    from torch.autograd import forward_ad
+    wq, ws, b = _weights(6, 8, 1)
+    x = torch.randn((3, 8), device=DEV)
+    image = torch.randn((1, 8, 2, 2), device=DEV)
+    ask = lambda t: t.clone().requires_grad_()                                                     # noqa: E731
+    for call in (lambda x, i, ws, b: pkg.int8_linear(x, wq, ws, b), lambda x, i, ws, b: pkg.int8_conv1x1(i, wq, ws, b)):
+        for args in ((ask(x), ask(image), ws, b), (x, image, ask(ws), b), (x, image, ws, ask(b))):
+            with pytest.raises(RuntimeError, match="no backward"):
+                call(*args)
+            with torch.no_grad():
+                call(*args)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))                               # noqa: E731
+        for grad in (True, False):               # (no_grad does not stop forward mode)
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: pkg.int8_linear(dual(x), wq, ws, b), lambda: pkg.int8_linear(x, wq, dual(ws), b),
+                             lambda: pkg.int8_linear(x, wq, ws, dual(b)), lambda: pkg.int8_conv1x1(dual(image), wq, ws, b),
+                             lambda: pkg.quantize_int8(dual(x))):
+                    with pytest.raises(RuntimeError, match="no backward"):
+                        call()
+                pkg.int8_linear(x, wq, ws, b)
