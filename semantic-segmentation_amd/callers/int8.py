@@ -18,6 +18,11 @@ def _norm(m):
     return type(m) is BatchNorm2d and m.running_mean is not None and not m.training
 
 
+def _runs_as(m, base):
+    """m runs `base`'s forward (a subclass with one of its own may take the layers in any other order)."""
+    return isinstance(m, base) and type(m).forward is base.forward and "forward" not in vars(m)
+
+
 def _convert_sequence(seq, min_channels):
     """Conv2d (BatchNorm2d) (ReLU) and Linear (ReLU) runs of a Sequential: one layer, the others become Identity."""
     names = list(seq._modules)
@@ -41,12 +46,12 @@ def _convert_sequence(seq, min_channels):
 def _convert(module, min_channels):
     if isinstance(module, _DcnConvBase):         # their inner convolutions place samples: left exact
         return
-    if isinstance(module, Bottleneck):
+    if _runs_as(module, Bottleneck):
         if _pointwise(module.conv1, min_channels) and _norm(module.bn1):
             module.conv1, module.bn1, module.relu1 = Int8Conv1x1.from_float(module.conv1, module.bn1, True), nn.Identity(), False
         if _pointwise(module.conv3, min_channels) and _norm(module.bn3):
             module.conv3, module.bn3 = Int8Conv1x1.from_float(module.conv3, module.bn3), nn.Identity()
-    elif isinstance(module, nn.Sequential):
+    elif _runs_as(module, nn.Sequential):
         _convert_sequence(module, min_channels)
     else:
         for name, m in module._modules.items():
@@ -62,7 +67,9 @@ def _convert(module, min_channels):
 def int8_inference(model, min_channels=16):
     """Converts `model` in place and returns it.  It has to be on the GPU and in eval mode: running statistics are folded
     into the weights, and the converted layers have no backward pass.  Layers with fewer than `min_channels` inputs are
-    left (a token's rounding costs as much as their product).  State dicts of the model change with its layers."""
+    left (a token's rounding costs as much as their product).  Norms and ReLUs join the layer before them in an
+    nn.Sequential and in a Bottleneck, but not in subclasses with a forward of their own; a Sequential is taken to be called
+    as a whole.  State dicts of the model change with its layers."""
     if model.training:
         raise RuntimeError("ddcn: int8_inference folds running statistics: call model.eval() first")
     if _pointwise(model, min_channels):
