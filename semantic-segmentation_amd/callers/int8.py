@@ -9,13 +9,23 @@ from ..dcn.deform_conv import _DcnConvBase
 from .resnet import Bottleneck
 
 
+def _plain(m, kind):
+    """A `kind` and no subclass, that runs its forward and nothing beside it: a hook would go with the layer, or see another."""
+    return type(m) is kind and "forward" not in vars(m) and \
+        not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
 def _pointwise(m, min_channels):
-    return (type(m) is nn.Conv2d and tuple(m.kernel_size) == (1, 1) and m.groups == 1 and m.stride[0] == m.stride[1]
+    return (_plain(m, nn.Conv2d) and tuple(m.kernel_size) == (1, 1) and m.groups == 1 and m.stride[0] == m.stride[1]
             and m.padding in ((0, 0), "valid") and m.in_channels >= min_channels)
 
 
+def _linear(m, min_channels):
+    return _plain(m, nn.Linear) and m.in_features >= min_channels
+
+
 def _norm(m):
-    return type(m) is BatchNorm2d and m.running_mean is not None and not m.training
+    return _plain(m, BatchNorm2d) and m.running_mean is not None and not m.training
 
 
 def _runs_as(m, base):
@@ -32,10 +42,10 @@ def _convert_sequence(seq, min_channels):
         if _pointwise(m, min_channels):
             norm = rest[0] if _norm(rest[0]) else None
             follows = 1 if norm is None else 2
-            relu = type(rest[follows - 1]) is nn.ReLU
+            relu = _plain(rest[follows - 1], nn.ReLU)
             seq._modules[name] = Int8Conv1x1.from_float(m, norm, relu)
-        elif type(m) is nn.Linear and m.in_features >= min_channels:
-            follows, relu = 1, type(rest[0]) is nn.ReLU
+        elif _linear(m, min_channels):
+            follows, relu = 1, _plain(rest[0], nn.ReLU)
             seq._modules[name] = Int8Linear.from_float(m, relu)
         else:
             continue
@@ -48,7 +58,9 @@ def _convert(module, min_channels):
         return
     if _runs_as(module, Bottleneck):
         if _pointwise(module.conv1, min_channels) and _norm(module.bn1):
-            module.conv1, module.bn1, module.relu1 = Int8Conv1x1.from_float(module.conv1, module.bn1, True), nn.Identity(), False
+            relu = _plain(module.relu, nn.ReLU)
+            module.conv1, module.bn1 = Int8Conv1x1.from_float(module.conv1, module.bn1, relu), nn.Identity()
+            module.relu1 = not relu
         if _pointwise(module.conv3, min_channels) and _norm(module.bn3):
             module.conv3, module.bn3 = Int8Conv1x1.from_float(module.conv3, module.bn3), nn.Identity()
     elif _runs_as(module, nn.Sequential):
@@ -57,7 +69,7 @@ def _convert(module, min_channels):
         for name, m in module._modules.items():
             if _pointwise(m, min_channels):
                 module._modules[name] = Int8Conv1x1.from_float(m)
-            elif type(m) is nn.Linear and m.in_features >= min_channels:
+            elif _linear(m, min_channels):
                 module._modules[name] = Int8Linear.from_float(m)
     for m in module._modules.values():
         if m is not None:
@@ -67,14 +79,14 @@ def _convert(module, min_channels):
 def int8_inference(model, min_channels=16):
     """Converts `model` in place and returns it.  It has to be on the GPU and in eval mode: running statistics are folded
     into the weights, and the converted layers have no backward pass.  Layers with fewer than `min_channels` inputs are
-    left (a token's rounding costs as much as their product).  Norms and ReLUs join the layer before them in an
-    nn.Sequential and in a Bottleneck, but not in subclasses with a forward of their own; a Sequential is taken to be called
-    as a whole.  State dicts of the model change with its layers."""
+    left (a token's rounding costs as much as their product), and so are layers with hooks.  Norms and ReLUs join the layer
+    before them in an nn.Sequential and in a Bottleneck, but not in subclasses with a forward of their own; a Sequential is
+    taken to be called as a whole.  State dicts of the model change with its layers."""
     if model.training:
         raise RuntimeError("ddcn: int8_inference folds running statistics: call model.eval() first")
     if _pointwise(model, min_channels):
         return Int8Conv1x1.from_float(model)
-    if type(model) is nn.Linear:
+    if _linear(model, 0):
         return Int8Linear.from_float(model)
     _convert(model, min_channels)
     return model

@@ -104,3 +104,52 @@ def test_plain_sequences_and_bottlenecks_are_folded(on_cpu):
     callers.int8_inference(seq), callers.int8_inference(block)
     assert [type(m).__name__ for m in seq] == ["Int8Conv1x1", "Identity", "Identity", "Int8Conv1x1", "Identity"]
     assert seq[0].relu and seq[3].relu and isinstance(block.bn1, nn.Identity) and not block.relu1
+
+
+def test_layers_with_hooks_stay_as_they_are(on_cpu):
+    """A hook sees the layer that it was put on: neither is it dropped with the layer, nor does a norm or an activation
+    that has one vanish into the layer before it."""
+    seen = []
+    hook = lambda m, *rest: seen.append(m)                                                         # noqa: E731
+    kinds = (lambda m: m.register_forward_hook(hook), lambda m: m.register_forward_pre_hook(hook),
+             lambda m: m.register_full_backward_hook(hook), lambda m: m.register_full_backward_pre_hook(hook))
+    x = torch.randn(1, 32, 2, 2)
+    for put in kinds:
+        for at in range(4):
+            seq = _fill_norms(nn.Sequential(nn.Conv2d(32, 32, 1), nn.BatchNorm2d(32), nn.ReLU(), nn.Conv2d(32, 16, 1)))
+            layer = seq[at]
+            put(layer)
+            callers.int8_inference(seq)
+            assert seq[at] is layer
+            names = [type(m).__name__ for m in seq]
+            assert names == [["Conv2d", "BatchNorm2d", "ReLU", "Int8Conv1x1"], ["Int8Conv1x1", "BatchNorm2d", "ReLU", "Int8Conv1x1"],
+                             ["Int8Conv1x1", "Identity", "ReLU", "Int8Conv1x1"], ["Int8Conv1x1", "Identity", "Identity", "Conv2d"]][at]
+            assert seq[0].relu is (at == 3) if at else True
+    for name in ("conv1", "bn1", "conv3", "bn3"):
+        block = _fill_norms(callers.Bottleneck(64, 16))
+        layer = getattr(block, name)
+        layer.register_forward_hook(hook)
+        callers.int8_inference(block)
+        assert getattr(block, name) is layer
+        other = "conv3" if name in ("conv1", "bn1") else "conv1"
+        assert type(getattr(block, other)).__name__ == "Int8Conv1x1" and type(getattr(block, "conv" + name[-1])) is nn.Conv2d
+        assert block.relu1 is (name in ("conv1", "bn1"))
+    # weights that a hook makes anew before every call
+    linear = torch.nn.utils.spectral_norm(nn.Linear(32, 8))
+    model = nn.ModuleDict(dict(fc=linear, other=nn.Linear(32, 8), last=nn.Conv2d(32, 8, 1))).eval()
+    model.last.forward = lambda x: x
+    callers.int8_inference(model)
+    assert model.fc is linear and type(model.other).__name__ == "Int8Linear" and type(model.last) is nn.Conv2d
+    alone = nn.Linear(32, 8).eval()
+    alone.register_forward_hook(hook)
+    assert callers.int8_inference(alone) is alone and x is not None
+
+
+def test_a_bottleneck_with_another_activation_keeps_it(on_cpu):
+    for relu in (nn.ReLU(), nn.SiLU()):
+        block = _fill_norms(callers.Bottleneck(64, 16))
+        block.relu = relu
+        if type(relu) is nn.ReLU:
+            relu.register_forward_hook(lambda m, i, o: None)
+        callers.int8_inference(block)
+        assert block.relu is relu and block.relu1 and not block.conv1.relu and isinstance(block.bn1, nn.Identity)
