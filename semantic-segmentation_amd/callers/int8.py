@@ -5,7 +5,9 @@ import torch.nn as nn
 from torch.nn.modules.batchnorm import BatchNorm2d
 
 from ..dcn import Int8Conv1x1, Int8Linear
+from ..dcn._lib import ELEMENT_TYPES
 from ..dcn.deform_conv import _DcnConvBase
+from ..dcn.int8 import MAX_CHANNELS, MAX_K
 from .resnet import Bottleneck
 
 
@@ -15,13 +17,18 @@ def _plain(m, kind):
         not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
 
 
+def _taken(m, k, channels, min_channels):
+    """The product takes a layer of this size and type."""
+    return max(min_channels, 1) <= k <= MAX_K and channels <= MAX_CHANNELS and m.weight.dtype in ELEMENT_TYPES
+
+
 def _pointwise(m, min_channels):
     return (_plain(m, nn.Conv2d) and tuple(m.kernel_size) == (1, 1) and m.groups == 1 and m.stride[0] == m.stride[1]
-            and m.padding in ((0, 0), "valid") and m.in_channels >= min_channels)
+            and m.padding in ((0, 0), "valid") and _taken(m, m.in_channels, m.out_channels, min_channels))
 
 
 def _linear(m, min_channels):
-    return _plain(m, nn.Linear) and m.in_features >= min_channels
+    return _plain(m, nn.Linear) and _taken(m, m.in_features, m.out_features, min_channels)
 
 
 def _norm(m):
@@ -79,9 +86,10 @@ def _convert(module, min_channels):
 def int8_inference(model, min_channels=16):
     """Converts `model` in place and returns it.  It has to be on the GPU and in eval mode: running statistics are folded
     into the weights, and the converted layers have no backward pass.  Layers with fewer than `min_channels` inputs are
-    left (a token's rounding costs as much as their product), and so are layers with hooks.  Norms and ReLUs join the layer
-    before them in an nn.Sequential and in a Bottleneck, but not in subclasses with a forward of their own; a Sequential is
-    taken to be called as a whole.  State dicts of the model change with its layers."""
+    left (a token's rounding costs as much as their product), and so are layers with hooks, in float64 or beyond the sizes
+    of `int8_linear`.  Norms and ReLUs join the layer before them in an nn.Sequential and in a Bottleneck, but not in
+    subclasses with a forward of their own; a Sequential is taken to be called as a whole.  State dicts of the model change
+    with its layers."""
     if model.training:
         raise RuntimeError("ddcn: int8_inference folds running statistics: call model.eval() first")
     if _pointwise(model, min_channels):

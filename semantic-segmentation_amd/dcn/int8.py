@@ -18,6 +18,7 @@ from . import _lib
 
 _F32 = torch.float32
 _INT8 = torch.int8
+MAX_K, MAX_CHANNELS = 131072, 1 << 20         # of ddcn_int8_product
 
 
 def _element_type(name, t):
@@ -121,7 +122,8 @@ def quantize_int8(x):
 
 def int8_linear(input, weight_q, weight_scale, bias=None, relu=False, out_dtype=None):
     """input [..., k] (float32, float16 or bfloat16), weight_q int8 [channels, k], weight_scale float32 [channels],
-    bias [channels] -> [..., channels] in `out_dtype` (the input's).  Rows of input may be strided."""
+    bias [channels] -> [..., channels] in `out_dtype` (the input's).  Rows of input may be strided.  k up to 131072, channels
+    up to 2^20, fewer than 2^31 tokens."""
     code = _element_type("input", input)
     shape = input.shape
     if not shape:

@@ -153,3 +153,25 @@ def test_a_bottleneck_with_another_activation_keeps_it(on_cpu):
             relu.register_forward_hook(lambda m, i, o: None)
         callers.int8_inference(block)
         assert block.relu is relu and block.relu1 and not block.conv1.relu and isinstance(block.bn1, nn.Identity)
+
+
+@pytest.mark.parametrize("make", [lambda: nn.Linear(131073, 4), lambda: nn.Conv2d(131073, 4, 1), lambda: nn.Linear(16, (1 << 20) + 1),
+                                  lambda: nn.Conv2d(16, (1 << 20) + 1, 1), lambda: nn.Linear(0, 4)],
+                         ids=["inputs", "input channels", "outputs", "output channels", "no inputs"])
+def test_layers_that_the_product_does_not_take_stay(on_cpu, make):
+    """They were met halfway through a model, after others had been converted."""
+    with torch.device("meta"):
+        far = make()
+    model = nn.Sequential(nn.Linear(32, 8), far).eval()
+    callers.int8_inference(model, min_channels=0)
+    assert type(model[0]).__name__ == "Int8Linear" and model[1] is far
+
+
+@pytest.mark.parametrize("make", [lambda: nn.Linear(32, 4), lambda: nn.Conv2d(32, 4, 1)], ids=["linear", "conv"])
+def test_double_layers_stay(on_cpu, make):
+    model = nn.ModuleList([nn.Linear(32, 8), make().double()]).eval()
+    callers.int8_inference(model)
+    assert type(model[0]).__name__ == "Int8Linear" and model[1].weight.dtype == torch.float64
+    bottleneck = _fill_norms(callers.Bottleneck(64, 16).double())
+    layers = list(bottleneck.modules())
+    assert list(callers.int8_inference(bottleneck).modules()) == layers
