@@ -150,3 +150,27 @@ def test_a_state_dict_that_is_refused_changes_nothing(calls, bits):
     empty = callers.AdamW(make(), bits=bits).state_dict()
     opt.load_state_dict(empty)
     assert not opt.state
+
+
+def test_a_first_step_that_is_refused_leaves_no_state():
+    """On a CPU model: NotImplementedError, and the optimizer is as new (the model may move to the GPU next)."""
+    params = _params(3, 300)
+    opt = callers.AdamW(params)
+    _give(params, {0, 1})
+    with pytest.raises(NotImplementedError):
+        opt.step()
+    assert not opt.state and not opt.state_dict()["state"]
+
+
+def test_a_later_step_that_is_refused_keeps_the_state(calls, monkeypatch):
+    params = _params(3, 300)
+    opt = callers.AdamW(params)
+    _give(params, {0, 1})
+    opt.step()
+
+    def refuse(*a, **kw):
+        raise RuntimeError("refused")
+    monkeypatch.setattr(optim, "adamw_step", refuse)
+    with pytest.raises(RuntimeError, match="refused"):
+        opt.step()
+    assert [opt.state[p]["step"] for p in params] == [1, 1]

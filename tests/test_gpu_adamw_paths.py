@@ -199,3 +199,16 @@ def test_norm_of_strided_gradients_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert float(out) == eager
+
+
+def test_a_model_that_moves_to_the_gpu_after_a_refused_step():
+    model = torch.nn.Linear(7, 5)
+    opt = callers.AdamW(model.parameters(), lr=LR)
+    for p in model.parameters():
+        p.grad = torch.ones_like(p)
+    with pytest.raises(NotImplementedError):
+        opt.step()
+    model.to(DEV)
+    before = [p.detach().clone() for p in model.parameters()]
+    opt.step()
+    assert all((p < b).all() for p, b in zip(model.parameters(), before)) and all(s["step"] == 1 for s in opt.state.values())
