@@ -7,6 +7,7 @@ i - 1 (`adamw_arena` gives the length).  In 8 bits `exp_avg` is int8, `exp_avg_s
 256 elements: 2.03 bytes a parameter instead of 8.  CPU tensors raise NotImplementedError; there is no fallback.
 """
 import ctypes
+import operator
 from array import array
 
 import torch
@@ -88,6 +89,19 @@ def _check_state(name, t, dtype, numel, device):
                            % (name, dtype, numel, t.dtype, t.numel()))
 
 
+def _step_numbers(step, count):
+    """-> (None or an array of `count` numbers, one number for all)"""
+    if hasattr(step, "__index__"):
+        step = operator.index(step)
+        if step >> 31:                  # an int of the C call would keep the low bits
+            raise RuntimeError("ddcn: step %d is below 1 or not below 2^31" % step)
+        return None, step
+    steps = array("i", step)
+    if len(steps) != count:
+        raise RuntimeError("ddcn: %d parameters but %d step numbers" % (count, len(steps)))
+    return steps, 1
+
+
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                exp_avg_scale=None, exp_avg_sq_scale=None, seed=None, grad_norm=None, max_norm=None):
     """One AdamW step over `params` (list of tensors of one type: float32, bfloat16 or float16), in place.  They are
@@ -149,11 +163,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
         raise RuntimeError("ddcn: max_norm and grad_norm go together")
     if grad_norm is not None and (grad_norm.dtype != torch.float32 or grad_norm.numel() != 1):
         raise RuntimeError("ddcn: grad_norm has to be one float32 value")
-    steps = None
-    if not hasattr(step, "__index__"):
-        steps, step = array("i", step), 1
-        if len(steps) != len(params):
-            raise RuntimeError("ddcn: %d parameters but %d step numbers" % (len(params), len(steps)))
+    steps, step = _step_numbers(step, len(params))
     if seed is None:
         seed = step if steps is None else sum(steps)
     hyper = _lib.AdamwHyper(lr, betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, step,

@@ -174,3 +174,12 @@ def test_a_later_step_that_is_refused_keeps_the_state(calls, monkeypatch):
     with pytest.raises(RuntimeError, match="refused"):
         opt.step()
     assert [opt.state[p]["step"] for p in params] == [1, 1]
+
+
+def test_step_numbers_beyond_32_bits_are_refused():
+    """2^32 + 1 would be step 1 in an int."""
+    for step in (1 << 31, (1 << 32) + 1, [1 << 31], -1, -(1 << 32) + 1):
+        with pytest.raises((RuntimeError, OverflowError)):
+            optim._step_numbers(step, 1)
+    assert optim._step_numbers(7, 1) == (None, 7) and optim._step_numbers(np.int64(7), 1) == (None, 7)
+    assert list(optim._step_numbers([7, 8], 2)[0]) == [7, 8]

@@ -212,3 +212,11 @@ def test_a_model_that_moves_to_the_gpu_after_a_refused_step():
     before = [p.detach().clone() for p in model.parameters()]
     opt.step()
     assert all((p < b).all() for p, b in zip(model.parameters(), before)) and all(s["step"] == 1 for s in opt.state.values())
+
+
+def test_step_numbers_that_do_not_fit_change_nothing():
+    p, g, m, v = (torch.ones(256, device=DEV) for _ in range(4))
+    for step in ((1 << 32) + 1, -(1 << 32) + 1, 1 << 31):
+        with pytest.raises(RuntimeError, match="below"):
+            callers.adamw_step([p], [g], m, v, step, LR)
+    assert all((t == 1).all() for t in (p, m, v))
