@@ -431,9 +431,9 @@ long long ddcn_adamw_arena(int count, const long long *numels)
     long long total = 0;
     for (int i = 0; i < count; ++i) {
         if (numels[i] < 0 || numels[i] > (1LL << 40)) return fail(DDCN_ERR_SHAPE, "tensor %d has %lld elements", i, numels[i]);
-        total += ceil_div(numels[i], kBlock) * kBlock;
+        total += ceil_div(numels[i], kBlock) * kBlock;         // (stays below 2^42)
+        if (total / kBlock >= (1LL << 32)) return fail(DDCN_ERR_UNSUPPORTED, "more than 2^40 elements in one arena");
     }
-    if (total / kBlock >= (1LL << 32)) return fail(DDCN_ERR_UNSUPPORTED, "more than 2^40 elements in one arena");
     return total;
 }
 

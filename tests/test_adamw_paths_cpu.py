@@ -183,3 +183,20 @@ def test_step_numbers_beyond_32_bits_are_refused():
             optim._step_numbers(step, 1)
     assert optim._step_numbers(7, 1) == (None, 7) and optim._step_numbers(np.int64(7), 1) == (None, 7)
     assert list(optim._step_numbers([7, 8], 2)[0]) == [7, 8]
+
+
+def _list(kind, values):
+    import ctypes
+    from array import array
+    a = array(kind, values)
+    return a, ctypes.c_void_p(a.buffer_info()[0])
+
+
+def test_arena_lengths_do_not_wrap():
+    """2^24 tensors of 2^40 elements and one of 256 are 2^64 + 256 together, which 64 bits hold as 256."""
+    keep, p = _list("q", [1 << 40] * (1 << 24) + [256])
+    assert _lib.lib().ddcn_adamw_arena(len(keep), p) == -5
+    keep, p = _list("q", [1 << 40, 1])
+    assert _lib.lib().ddcn_adamw_arena(2, p) == -5 and _lib.lib().ddcn_adamw_arena(1, p) == -5
+    keep, p = _list("q", [(1 << 40) - 512, 256])
+    assert _lib.lib().ddcn_adamw_arena(2, p) == (1 << 40) - 256
