@@ -557,6 +557,7 @@ int ddcn_adamw_moments(const void *exp_avg, const void *exp_avg_sq, const float 
 
 size_t ddcn_grad_norm_workspace_bytes(int count, const long long *numels)
 {
+    if (count < 0 || (count && !numels)) return 0;
     long long chunks = 0;
     for (int i = 0; i < count; ++i) chunks += ceil_div(numels[i] > 0 ? numels[i] : 0, kNormChunk);
     return round_up((size_t)(chunks > 0 ? chunks : 1) * sizeof(double), 256);

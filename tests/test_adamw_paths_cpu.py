@@ -200,3 +200,11 @@ def test_arena_lengths_do_not_wrap():
     assert _lib.lib().ddcn_adamw_arena(2, p) == -5 and _lib.lib().ddcn_adamw_arena(1, p) == -5
     keep, p = _list("q", [(1 << 40) - 512, 256])
     assert _lib.lib().ddcn_adamw_arena(2, p) == (1 << 40) - 256
+
+
+def test_norm_workspace_of_a_list_that_is_not_there():
+    L = _lib.lib()
+    assert L.ddcn_grad_norm_workspace_bytes(3, None) == 0 and L.ddcn_grad_norm_workspace_bytes(-1, None) == 0
+    assert L.ddcn_grad_norm_workspace_bytes(0, None) == 256
+    keep, p = _list("q", [100])
+    assert L.ddcn_grad_norm_workspace_bytes(1, p) == 256
