@@ -208,3 +208,17 @@ def test_norm_workspace_of_a_list_that_is_not_there():
     assert L.ddcn_grad_norm_workspace_bytes(0, None) == 256
     keep, p = _list("q", [100])
     assert L.ddcn_grad_norm_workspace_bytes(1, p) == 256
+
+
+@pytest.mark.parametrize("root", [0.3, 1.5, 10.25, 100.9])
+def test_codes_are_right_on_average_and_what_they_stand_for_is_not(root):
+    """q = floor(t + u) has the mean t, and q^2 the mean t^2 + f (1 - f), f the fraction of t: what include/ddcn_hip.h states of
+    the decoded moments.  Over N places q is n + 1 with probability f, n otherwise: 5 sigma of both means, and u's 2^-16 steps."""
+    n, whole = 1 << 16, np.floor(root)
+    f = root - whole
+    for u in ref.noise(np.arange(n), 11):
+        q = np.floor((np.float32(root) + u).astype(np.float32)).astype(np.float64)
+        sigma = np.sqrt(f * (1 - f) / n)
+        assert abs(q.mean() - root) < 5 * sigma + 2.0 ** -15
+        assert abs((q * q).mean() - (root ** 2 + f * (1 - f))) < (2 * whole + 1) * (5 * sigma + 2.0 ** -15)
+    assert f * (1 - f) > (2 * whole + 1) * 5 * sigma or root > 100       # it tells the two apart
