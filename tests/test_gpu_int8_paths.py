@@ -76,3 +76,39 @@ def test_gradients_asked_for_are_refused_not_dropped():
                     with pytest.raises(RuntimeError, match="no backward"):
                         call()
                 pkg.int8_linear(x, wq, ws, b)
+
+
+# the tiled product (more than 512 tokens, K too short to be split): 64 x 64 tiles, and 128 x 128 where they fill the CUs
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("off", [0, 1, 5])
+@pytest.mark.parametrize("images,h,w,k,n,nchw", [(1, 700, 1, 100, 65, 0), (1, 1500, 1, 64, 129, 0), (1, 1003, 1, 200, 523, 0), (1, 601, 1, 65, 7, 0),
+                                                 (1, 12503, 1, 130, 265, 0), (1, 13000, 1, 64, 512, 0),
+                                                 (2, 23, 25, 100, 33, 1), (2, 23, 25, 64, 130, 1), (3, 15, 15, 65, 64, 1), (90, 3, 3, 64, 40, 1),
+                                                 (700, 1, 1, 64, 40, 1), (2, 97, 97, 64, 130, 1), (2, 97, 97, 200, 256, 1), (5, 61, 67, 64, 129, 1),
+                                                 (200, 9, 11, 64, 128, 1), (2, 96, 98, 64, 131, 1)])
+def test_stores_of_tiles_at_any_address(images, h, w, k, n, nchw, dtype, off):
+    """Rows and planes of odd length, images that end inside a run of eight, outputs from any element on: every element, and
+    the memory on both sides."""
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(k + n)
+    x = torch.randn((images * h * w, k), generator=g).to(t).to(DEV)
+    wq, ws, b = _weights(n, k, n)
+    total, edge = images * h * w * n, 64
+    big = torch.full((edge + off + total + edge,), 7.5, dtype=t, device=DEV)
+    y = big[edge + off:edge + off + total]
+    if nchw:
+        x = x.view(images, h * w, k).transpose(1, 2).contiguous()
+        geom = _lib.Int8Geom(images, h, w, k, n, 1, _lib.ELEMENT_TYPES[t], _lib.ELEMENT_TYPES[t], 0, k * h * w, w, 1, h * w, k)
+    else:
+        geom = _lib.Int8Geom(images, h, w, k, n, 0, _lib.ELEMENT_TYPES[t], _lib.ELEMENT_TYPES[t], 0, 0, k, 0, 1, k)
+    size = _lib.lib().ddcn_int8_workspace_bytes(geom)
+    work = torch.empty(size, dtype=torch.uint8, device=DEV)
+    _lib.check(_lib.lib().ddcn_int8_product(_lib.ptr(x), _lib.ptr(wq), _lib.ptr(ws), _lib.ptr(b), _lib.ptr(y), _lib.ptr(work), size, geom,
+                                            _lib.stream_of(0)))
+    assert (big[:edge + off] == 7.5).all() and (big[edge + off + total:] == 7.5).all()
+    tokens = _np(x.transpose(1, 2).reshape(-1, k) if nchw else x)
+    want, tol = ref.product(tokens, _np(wq), _np(ws), _np(b))
+    half = torch.finfo(t).eps / 2 if t != torch.float32 else 0.0
+    tol = tol + half * (np.abs(want) + tol) + (2.0 ** -25 if t == torch.float16 else 0)
+    got = _np(y.view(images, n, h * w).transpose(1, 2) if nchw else y).reshape(-1, n)
+    assert (np.abs(got - want) <= tol).all(), np.argwhere(~(np.abs(got - want) <= tol))[:10]
