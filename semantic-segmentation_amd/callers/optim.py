@@ -142,7 +142,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
     if given < len(grads) or not contiguous or not grad_contiguous or numels != grad_numels:
         wrong = _lib.tensors().alike(params, grads)
         if wrong == 1:
-            raise RuntimeError("ddcn: parameters have to be contiguous (or channels-last), gradients in the same order")
+            raise RuntimeError("ddcn: parameters have to be contiguous (or channels-last), gradients of their shapes in the "
+                               "same order")
         if wrong == 2:
             raise RuntimeError("ddcn: a gradient has another number of elements than its parameter")
     if not distinct:

@@ -104,7 +104,7 @@ PyObject *changed(PyObject *, PyObject *args)
     });
 }
 
-// alike(params, grads) -> 0, or what is wrong with a pair (a None among the gradients is none): 1, another order in memory, or
+// alike(params, grads) -> 0, or what is wrong with a pair (a None among the gradients is none): 1, another shape or order in memory, or
 // one that is neither contiguous nor channels-last; 2, another number of elements
 PyObject *alike(PyObject *, PyObject *args)
 {
@@ -121,8 +121,9 @@ PyObject *alike(PyObject *, PyObject *args)
             const at::Tensor *p = tensor_of(PyList_GET_ITEM(params, i)), *g = p ? tensor_of(PyList_GET_ITEM(grads, i)) : nullptr;
             if (!g) return nullptr;
             if (!p->is_contiguous() || !g->is_contiguous())
-                wrong = p->strides() == g->strides() && (p->is_contiguous() || p->is_contiguous(at::MemoryFormat::ChannelsLast) ||
-                                                         p->is_contiguous(at::MemoryFormat::ChannelsLast3d)) ? 0 : 1;
+                wrong = p->sizes() == g->sizes() && p->strides() == g->strides() &&
+                        (p->is_contiguous() || p->is_contiguous(at::MemoryFormat::ChannelsLast) ||
+                         p->is_contiguous(at::MemoryFormat::ChannelsLast3d)) ? 0 : 1;
             if (!wrong && p->numel() != g->numel()) wrong = 2;
         }
         return PyLong_FromLong(wrong);

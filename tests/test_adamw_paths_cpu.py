@@ -222,3 +222,16 @@ def test_codes_are_right_on_average_and_what_they_stand_for_is_not(root):
         assert abs(q.mean() - root) < 5 * sigma + 2.0 ** -15
         assert abs((q * q).mean() - (root ** 2 + f * (1 - f))) < (2 * whole + 1) * (5 * sigma + 2.0 ** -15)
     assert f * (1 - f) > (2 * whole + 1) * 5 * sigma or root > 100       # it tells the two apart
+
+
+def test_equal_strides_of_other_shapes_are_not_alike():
+    """A step reads as many elements in a row as the parameter has: a gradient of equal strides and number of elements whose
+    shape is another one may end before (here after 60 of 108), or lie elsewhere."""
+    t = _lib.tensors()
+    p = torch.zeros(2, 6, 3, 3).to(memory_format=torch.channels_last)
+    g = torch.zeros(200).as_strided((1, 12, 3, 3), p.stride())
+    assert g.stride() == p.stride() and g.numel() == p.numel() and t.alike([p], [g]) == 1
+    p = torch.zeros(2, 6)
+    g = torch.zeros(3, 6)[:, :4]
+    assert g.stride() == p.stride() and g.numel() == p.numel() and t.alike([p], [g]) == 1
+    assert t.alike([p], [torch.zeros(12)]) == 0 and t.alike([p], [torch.zeros(3, 4)]) == 0       # one run of memory each
