@@ -225,7 +225,10 @@ class _Arena:
         for p in params:
             n = p.numel()
             end = start + -(-n // BLOCK) * BLOCK
-            shaped = lambda t: torch.as_strided(t, p.shape, p.stride(), start)                   # noqa: E731, B023
+            if _dense(p):
+                shaped = lambda t: torch.as_strided(t, p.shape, p.stride(), start)               # noqa: E731, B023
+            else:                    # it can have no step; its strides may reach beyond its part
+                shaped = lambda t: t[start:start + n].view(p.shape)                              # noqa: E731, B023
             state = dict(exp_avg=shaped(self.exp_avg), exp_avg_sq=shaped(self.exp_avg_sq))
             state.update({k: t[start // BLOCK:end // BLOCK] for k, t in self.scales.items()})
             yield state
@@ -322,7 +325,7 @@ class AdamW(torch.optim.Optimizer):
         if not types or any(t.shape != p.shape for t in moments) or any(t.shape != (-(-p.numel() // BLOCK),) for t in scales):
             raise ValueError("the state dict holds %s, not the state of AdamW with bits=%d over these parameters"
                              % (found, self.bits))
-        if self.bits == 8 and not all(_same_order(t, p) for t in moments):      # codes and their scales go by memory
+        if self.bits == 8 and _dense(p) and not all(_same_order(t, p) for t in moments):      # codes and their scales go by memory
             raise ValueError("8-bit moments of a parameter in another memory format")
         if int(saved["step"]) < 0:
             raise ValueError("step number %r" % (saved["step"],))

@@ -235,3 +235,23 @@ def test_equal_strides_of_other_shapes_are_not_alike():
     g = torch.zeros(3, 6)[:, :4]
     assert g.stride() == p.stride() and g.numel() == p.numel() and t.alike([p], [g]) == 1
     assert t.alike([p], [torch.zeros(12)]) == 0 and t.alike([p], [torch.zeros(3, 4)]) == 0       # one run of memory each
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_of_frozen_parameters_of_any_strides_are_their_own(calls, bits):
+    """A parameter that is no run of memory can have no step, but it may lie, frozen, beside others."""
+    frozen = [torch.zeros(40, 60)[:, ::2], torch.zeros(30, 20).t(), torch.zeros(5, 6, 7, 8)[:, :, 1:5], torch.zeros(1, 1).expand(9, 300)]
+    params = [p for t in frozen for p in (*_params(3), torch.nn.Parameter(t))] + _params(5)
+    opt = callers.AdamW(params, bits=bits)
+    _give(params, {0, 2, 4, 6, 8})
+    opt.step()
+    for i, p in enumerate(params):
+        for k, t in opt.state[p].items():
+            if k != "step":
+                t.fill_(i + 1)
+    for i, p in enumerate(params):
+        assert all((t == i + 1).all() and (k.endswith("scale") or t.shape == p.shape) for k, t in opt.state[p].items() if k != "step")
+    again = callers.AdamW(params, bits=bits)
+    again.load_state_dict(opt.state_dict())
+    for i, p in enumerate(params):
+        assert all((t == i + 1).all() for k, t in again.state[p].items() if k != "step")
