@@ -238,8 +238,9 @@ __device__ __forceinline__ void update_block(const AdamwArgs &a, const Place &w,
 
 // U blocks per wave, one after the other in the arena; where all of them are whole, every load is issued before the first
 // result is needed.  Every byte moves once.  fp32 moments, 28 bytes an element: bound by HBM, 39.6 M elements in 185 us, 6.0
-// TB/s.  8-bit ones, 16 bytes an element: 106 us for the same, 6.0 TB/s.  With bf16 parameters too, 10 bytes an element, its
-// 100 VALU instructions -- decoding, hash, two roots and their rounding -- bound it: 45 M elements in 113 us, 4.0 TB/s.
+// TB/s.  8-bit ones, 16 bytes an element: 105 to 118 us for the same, 6.0 to 5.4 TB/s.  With bf16 parameters too, 10 bytes an
+// element, its 100 VALU instructions -- decoding, hash, two roots and their rounding -- bound it: 45 M elements in 113 to 122 us,
+// 4.0 TB/s.
 template <int DT, int BITS, int U>
 __global__ __launch_bounds__(64 * kWaves) void adamw_kernel(const AdamwArgs a)
 {
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(1024) void norm_final_kernel(const double *partial,
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // Blocks per wave.  fp32 moments: one (the large launch of ResNet-50's 41 M parameters takes 185 us, 190 with two or four).
-// 8 bits: two, whose loads then hide behind the other's arithmetic (107 us; 123 with one, 110 with four) -- but one where
+// 8 bits: two, whose loads then hide behind the other's arithmetic (107 us; 123 with one, 110 with four, in turn) -- but one where
 // two would leave CUs without work.
 constexpr unsigned kSpreadBlocks = 8192;
 // Blocks of tensors without a gradient that a launch may hold between two others, as one entry whose waves end at once: below,
