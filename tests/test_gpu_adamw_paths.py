@@ -220,3 +220,35 @@ def test_step_numbers_that_do_not_fit_change_nothing():
         with pytest.raises(RuntimeError, match="below"):
             callers.adamw_step([p], [g], m, v, step, LR)
     assert all((t == 1).all() for t in (p, m, v))
+
+
+def test_a_parameter_of_more_than_2_31_elements():
+    """It goes in pieces; a small tensor behind it, and one without a gradient before that.  Elements at the ends of the
+    pieces against a call over them alone."""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 60e9:
+        pytest.skip("needs 60 GB")
+    big, small = (1 << 31) + 5000, 700
+    p, g = torch.zeros(big, dtype=torch.bfloat16, device=DEV), torch.zeros(big, dtype=torch.bfloat16, device=DEV)
+    q, h = (torch.randn(small, generator=_rng(70 + i)).to(torch.bfloat16).to(DEV) for i in range(2))
+    parts = [slice(0, 512), slice((1 << 31) - 512, (1 << 31) + 512), slice(big - 904, big)]
+    for i, at in enumerate(parts):
+        p[at], g[at] = (torch.randn(at.stop - at.start, generator=_rng(80 + 2 * i + j)).to(torch.bfloat16).to(DEV) for j in range(2))
+    alone = [p[at].clone() for at in parts] + [q.clone()]
+    grads = [g[at].clone() for at in parts] + [h]
+    idle = torch.zeros(300, dtype=torch.bfloat16, device=DEV)
+    n = callers.adamw_arena([p, idle, q])
+    m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    k = callers.adamw_arena(alone)
+    m2, v2 = torch.zeros(k, device=DEV), torch.zeros(k, device=DEV)
+    for t in (1, 2):
+        callers.adamw_step([p, idle, q], [g, None, h], m, v, t, LR, BETAS, EPS, WD)
+        callers.adamw_step(alone, grads, m2, v2, t, LR, BETAS, EPS, WD)
+    start = ref.starts_of([big, 300, small])[0]
+    places = parts + [slice(start[2], start[2] + small)]
+    for at, x, a in zip(places, alone, ref.starts_of([x.numel() for x in alone])[0]):
+        size = x.numel()
+        assert torch.equal(m[at], m2[a:a + size]) and torch.equal(v[at], v2[a:a + size]) and x.any()
+    for at, x in zip(parts, alone):
+        assert torch.equal(p[at], x)
+    assert torch.equal(q, alone[3]) and not idle.any() and not m[start[1]:start[2]].any() and not p[4096:1 << 20].any()
