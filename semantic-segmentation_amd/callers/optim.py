@@ -239,9 +239,10 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's interface over `adamw_step`.
 
     bits=32 or 8: how the moments are held (in 8 bits those of elements far below the largest of their 256 settle too high:
-    the first moment by 5 % at a thousandth of it, 30 % at a ten-thousandth; include/ddcn_hip.h).  max_norm: clip all gradients by their global norm first (the last norm is
-    kept in `last_grad_norm`, a scalar on the GPU); a step whose norm is not finite changes no parameter and no moment,
-    though its step number counts.  seed: of the rounding of 8-bit moments; the same seed repeats a run.
+    the first moment by 5 % at a thousandth of it, 30 % at a ten-thousandth; include/ddcn_hip.h).  max_norm: clip all
+    gradients by their global norm first (the last norm is kept in `last_grad_norm`, a scalar on the GPU); a step whose norm
+    is not finite changes no parameter and no moment, though its step number counts.  seed: of the rounding of 8-bit
+    moments; the same seed repeats a run.
     Parameters of one group may have different types (one arena each); all live on one GPU."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, max_norm=None, seed=0):
