@@ -294,13 +294,14 @@ class AdamW(torch.optim.Optimizer):
             first = (g, dtype) not in self._arenas
             group, arena, state = self.param_groups[g], self._arena(g, dtype, params), self.state
             steps = [state[p]["step"] + (x is not None) for p, x in zip(params, gs)]
-            live = {s for s, x in zip(steps, gs) if x is not None}       # the others' numbers do not count
+            counts = {steps[0]} if steps.count(steps[0]) == len(steps) else \
+                {s for s, x in zip(steps, gs) if x is not None}          # the others' numbers do not count
             # a seed for every step and arena: the sum of an arena's step numbers grows at each of its steps (their maximum
             # does not, where the gradients belong to tensors that have made fewer), and it comes back with a state dict
             seed = self.seed + 0x10001 * number + 0x3779B1 * sum(steps)
             try:
                 adamw_step(params, gs, arena.exp_avg, arena.exp_avg_sq,
-                           live.pop() if len(live) == 1 else [max(s, 1) for s in steps], group["lr"],
+                           counts.pop() if len(counts) == 1 else [max(s, 1) for s in steps], group["lr"],
                            group["betas"], group["eps"], group["weight_decay"], seed=seed, grad_norm=norm,
                            max_norm=self.max_norm, **arena.scales)
             except Exception:
